@@ -340,6 +340,96 @@ enum nbh_xoro_kind { NBH_XORO_NEXT = 0, NBH_XORO_JUMP = 1, NBH_XORO_UNIFORM_F32 
                      NBH_XORO_NORMAL_F32 = 4, NBH_XORO_NORMAL_F64 = 5 };
 int nbh_xoro_one(void *state, int kind, void *out, nbh_stream_t stream);
 
+/* ---- rows of logits -------------------------------------------------------- */
+
+/* Operators over the last axis of a rows x vocab array of float32, float16 or bfloat16
+ * whose items lie next to each other within a row; rows are `stride` bytes apart (any
+ * sign, any alignment the items allow; 0 repeats a row of an input).  vocab < 2^31.
+ * Integer arrays are 4 or 8 bytes per item, as their `_bytes` argument says.  All work is
+ * asynchronous on `stream`; nothing is allocated.  Temperatures are 1e-30 to 1e30. */
+enum nbh_row_dtype { NBH_ROW_F32 = 0, NBH_ROW_F16 = 1, NBH_ROW_BF16 = 2 };
+
+/* Penalties for repeated tokens, biases and a mask.  For entry v of row r, with
+ * h = tokens[offsets[r] .. offsets[r + 1]) the row's history, of which the first
+ * prompts[r] tokens are the prompt (none without `prompts`):
+ *   x = logits[r, v]
+ *   v in h:            x = x > 0 ? x / repetition : x * repetition
+ *   c times behind the prompt, c > 0:  x = (x - frequency * c) - presence
+ *   (v, b) among bias_tokens / bias_values[bias_offsets[r] .. bias_offsets[r + 1]), the
+ *   last such pair:    x = x + b
+ *   out[r, v] = bit v % 32 of word v / 32 of the row's mask set (or no mask) ? x : -inf
+ * in float32, rounded once.  Tokens outside [0, vocab) are skipped, offsets are clamped
+ * to the arrays.  `repetition`, `presence`, `frequency`: one float32 per row, or NULL for
+ * the value beside them.  `out` is of the logits' type or float32 and may be the logits
+ * themselves.  Fewer than 2^31 tokens and pairs. */
+struct nbh_logits_adjust_args {
+    int64_t struct_bytes;              /* sizeof(struct nbh_logits_adjust_args) */
+    const void *logits;
+    void *out;
+    int64_t rows, vocab, in_stride, out_stride, dtype, out_dtype;
+    const void *tokens, *offsets, *prompts;
+    int64_t n_tokens, token_bytes, offset_bytes, prompt_bytes;
+    const float *repetition, *presence, *frequency;
+    double repetition_value, presence_value, frequency_value;
+    const void *bias_tokens, *bias_offsets;
+    const float *bias_values;
+    int64_t n_bias, bias_token_bytes, bias_offset_bytes;
+    const void *mask;
+    int64_t mask_stride;
+};
+int nbh_logits_adjust(const struct nbh_logits_adjust_args *args, nbh_stream_t stream);
+
+/* The k largest entries of each row, largest first: values[r, j] = logits[r, indices[r, j]].
+ * NaN counts as larger than everything, -0 and +0 as equal; equal entries come in the order
+ * of their indices.  lse (or NULL): log sum exp(logits[r, :] / temperature).
+ * 1 <= k <= min(vocab, NBH_ROW_TOP_MOST).  `workspace` holds
+ * nbh_rows_top_workspace(rows, vocab, k, dtype) bytes (none when that is 0), 16-byte
+ * aligned, used by one call at a time. */
+#define NBH_ROW_TOP_MOST 1024
+size_t nbh_rows_top_workspace(int64_t rows, int64_t vocab, int64_t k, int dtype);
+int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int64_t stride, int dtype, int64_t k, void *values,
+                 int64_t values_stride, int32_t *indices, int64_t indices_stride, float *lse, double temperature,
+                 void *workspace, size_t workspace_bytes, nbh_stream_t stream);
+
+/* Distillation from the k entries a teacher gives for each row (values of the teacher's
+ * type, indices into the student's vocabulary; an entry whose index is outside
+ * [0, vocab) or whose value is -inf is absent; an index may occur more than once):
+ *   lse = log sum exp(student[r, :] / T),  log q(v) = student[r, v] / T - lse
+ *   p_j = exp(values[r, j] / T - teacher_lse[r]), or without `teacher_lse` the softmax of
+ *         values[r, :] / T over the entries present
+ *   loss[r] = sum p_j (log p_j - log q(indices[r, j]))          entries of p_j = 0 count 0
+ *   grad[r, v] = grad_loss[r] / T * (q(v) sum p_j - sum over indices[r, j] = v of p_j)
+ * A row with no entry present has loss 0 and gradient 0, one with grad_loss 0 gradient 0.
+ * `what`: NBH_DISTILL_LOSS writes loss and lse (lse may be NULL), NBH_DISTILL_GRAD writes
+ * grad from the lse it is given, their sum does both at once.  grad is of the student's
+ * type and may be the student's logits themselves.  k <= NBH_ROW_TOP_MOST.  `workspace` as
+ * above, nbh_rows_distill_workspace(rows, vocab, k, dtype, what) bytes. */
+enum nbh_distill_what { NBH_DISTILL_LOSS = 1, NBH_DISTILL_GRAD = 2 };
+struct nbh_rows_distill_args {
+    int64_t struct_bytes;              /* sizeof(struct nbh_rows_distill_args) */
+    int64_t what;
+    const void *student;
+    int64_t rows, vocab, stride, dtype;
+    const void *values, *indices;
+    int64_t k, values_stride, values_dtype, indices_stride, index_bytes;
+    const float *teacher_lse, *grad_loss;
+    int64_t grad_loss_stride;          /* bytes from row to row; 0: one number for all rows */
+    double grad_loss_value;            /* in place of grad_loss, when that is NULL */
+    double temperature;
+    float *loss, *lse;
+    void *grad;
+    int64_t grad_stride;
+    void *workspace;
+    int64_t workspace_bytes;
+};
+size_t nbh_rows_distill_workspace(int64_t rows, int64_t vocab, int64_t k, int dtype, int what);
+int nbh_rows_distill(const struct nbh_rows_distill_args *args, nbh_stream_t stream);
+
+/* *capturing = 1 if `stream` is being captured into a graph, else 0. */
+int nbh_stream_is_capturing(nbh_stream_t stream, int *capturing);
+/* *dev = the device whose memory `address` lies in. */
+int nbh_pointer_device(const void *address, int *dev);
+
 #ifdef __cplusplus
 }
 #endif

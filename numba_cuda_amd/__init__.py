@@ -22,10 +22,11 @@ if config.ENABLE_CUDASIM:
     from numba_cuda_amd import simulator as _simulator
     from numba_cuda_amd.simulator import *  # noqa: F401,F403
     from numba_cuda_amd.simulator import (_auto_device, _contiguous_strides_like_array,  # noqa: F401
-                                          _order_like_array, devicearray, random, reduction)
+                                          _order_like_array, devicearray, logits, random, reduction)
     # modules a user may import by name get the CPU mode's versions
     for _name, _module in (("random", "simulator.random"), ("api", "simulator"), ("args", "simulator.args"),
                            ("kernels.reduction", "simulator.reduction"), ("kernels.transpose", "simulator.transpose"),
+                           ("kernels.logits", "simulator.logits"),
                            ("cudadrv.devicearray", "simulator.hostarray")):
         _sys.modules[__name__ + "." + _name] = _sys.modules[__name__ + "." + _module]
     reduce = Reduce  # noqa: F405
@@ -47,6 +48,7 @@ else:
     from numba_cuda_amd import kernels  # noqa: F401
     from numba_cuda_amd.kernels import reduction  # noqa: F401  (the reference exposes the module as cuda.reduction)
     from numba_cuda_amd.kernels import transpose as _transpose  # noqa: F401
+    from numba_cuda_amd.kernels import logits  # noqa: F401
     from numba_cuda_amd.kernels.reduction import Reduce
     from numba_cuda_amd import random  # noqa: F401
 

@@ -87,6 +87,15 @@ SIGNATURES = {
     "nbh_xoro_normal_f32": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp]),
     "nbh_xoro_normal_f64": (c_int, [c_vp, c_i64, c_vp, c_i64, c_vp]),
     "nbh_xoro_one": (c_int, [c_vp, c_int, c_vp, c_vp]),
+    # the two argument structures are packed into bytes (kernels/logits.py)
+    "nbh_logits_adjust": (c_int, [c_char_p, c_vp]),
+    "nbh_rows_top_workspace": (c_size, [c_i64, c_i64, c_i64, c_int]),
+    "nbh_rows_top": (c_int, [c_vp, c_i64, c_i64, c_i64, c_int, c_i64, c_vp, c_i64, c_vp, c_i64, c_vp, ctypes.c_double,
+                             c_vp, c_size, c_vp]),
+    "nbh_rows_distill_workspace": (c_size, [c_i64, c_i64, c_i64, c_int, c_int]),
+    "nbh_rows_distill": (c_int, [c_char_p, c_vp]),
+    "nbh_stream_is_capturing": (c_int, [c_vp, P(c_int)]),
+    "nbh_pointer_device": (c_int, [c_vp, P(c_int)]),
 }
 
 # enum nbh_dtype / enum nbh_op

@@ -1,0 +1,174 @@
+// Helpers of the kernels that work on the rows of a 2-d array of logits (logits.hip, toprows.hip,
+// distill.hip): 16-byte vectors of float32, float16 or bfloat16 at any element alignment, and the
+// running maximum and sum of a softmax.
+#pragma once
+
+#include <float.h>
+
+#include "common.h"
+
+typedef float nbh_f32x4 __attribute__((ext_vector_type(4)));
+typedef float nbh_f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 nbh_f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 nbh_bf16x2 __attribute__((ext_vector_type(2)));
+
+// Workgroups of one launch: with up to 1024 lanes each they stay below 2^32 lanes.  2^31 entries of a row
+// make 2^19 tiles of 4096, so every row fits a launch.
+#define NBH_ROW_MOST_GROUPS (1 << 21)
+
+// Element types.  `items` elements make 16 bytes; arithmetic is float32 throughout, stores round once,
+// to nearest even.
+struct nbh_row_f32 {
+    typedef float item;
+    static constexpr int items = 4;
+    static __device__ __forceinline__ float get(item x) { return x; }
+    static __device__ __forceinline__ item put(float x) { return x; }
+    static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[4])
+    {
+        for (int i = 0; i < 4; ++i)
+            f[i] = __uint_as_float(v[i]);
+    }
+    static __device__ __forceinline__ nbh_u32x4 pack(const float (&f)[4])
+    {
+        nbh_u32x4 v;
+        for (int i = 0; i < 4; ++i)
+            v[i] = __float_as_uint(f[i]);
+        return v;
+    }
+};
+struct nbh_row_f16 {
+    typedef _Float16 item;
+    static constexpr int items = 8;
+    static __device__ __forceinline__ float get(item x) { return (float)x; }
+    static __device__ __forceinline__ item put(float x) { return (item)x; }
+    static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[8])
+    {
+        for (int i = 0; i < 4; ++i) {
+            const nbh_f16x2 h = __builtin_bit_cast(nbh_f16x2, (uint32_t)v[i]);
+            f[2 * i] = (float)h[0];
+            f[2 * i + 1] = (float)h[1];
+        }
+    }
+    static __device__ __forceinline__ nbh_u32x4 pack(const float (&f)[8])
+    {
+        nbh_u32x4 v;
+        for (int i = 0; i < 4; ++i) {
+            const nbh_f16x2 h = {(_Float16)f[2 * i], (_Float16)f[2 * i + 1]};
+            v[i] = __builtin_bit_cast(uint32_t, h);
+        }
+        return v;
+    }
+};
+struct nbh_row_bf16 {
+    typedef uint16_t item;
+    static constexpr int items = 8;
+    static __device__ __forceinline__ float get(item x) { return __uint_as_float((uint32_t)x << 16); }
+    static __device__ __forceinline__ item put(float x)
+    {
+        return __builtin_bit_cast(uint16_t, (__bf16)x);
+    }
+    static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[8])
+    {
+        for (int i = 0; i < 4; ++i) {
+            f[2 * i] = __uint_as_float(v[i] << 16);
+            f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ nbh_u32x4 pack(const float (&f)[8])
+    {
+        nbh_u32x4 v;
+        for (int i = 0; i < 4; ++i) {
+            const nbh_f32x2 two = {f[2 * i], f[2 * i + 1]};
+            v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(two, nbh_bf16x2));
+        }
+        return v;
+    }
+};
+
+// The 16 bytes at element `at` of a row of `n` elements; elements behind the row's end read as `fill`.
+template <typename E, bool NT>
+__device__ __forceinline__ void nbh_row_load(const typename E::item *row, int64_t at, int64_t n, float fill,
+                                             float (&f)[E::items])
+{
+    if (at + E::items <= n) {
+        E::unpack(nbh_load16<sizeof(typename E::item), NT>(row + at), f);
+    } else {
+        for (int i = 0; i < E::items; ++i)
+            f[i] = at + i < n ? E::get(row[at + i]) : fill;
+    }
+}
+template <typename E, bool NT>
+__device__ __forceinline__ void nbh_row_store(typename E::item *row, int64_t at, int64_t n, const float (&f)[E::items])
+{
+    if (at + E::items <= n) {
+        nbh_store16<sizeof(typename E::item), NT>(row + at, E::pack(f));
+    } else {
+        for (int i = 0; i < E::items; ++i)
+            if (at + i < n)
+                row[at + i] = E::put(f[i]);
+    }
+}
+
+// Running softmax statistics: `peak` is the largest value so far, kept finite so that no difference of
+// infinities arises, `sum` is sum 2^((x - peak) * scale) with scale = log2(e) / temperature.  Subtracting
+// before scaling keeps the exponent exact at the peak, also for rows filled with the type's lowest value.
+// A NaN stays in `sum`; a row of -inf has sum 0; +inf makes it inf.
+struct nbh_softmax {
+    float peak, sum;
+};
+__device__ __forceinline__ nbh_softmax nbh_softmax_empty() { return {-FLT_MAX, 0.0f}; }
+__device__ __forceinline__ float nbh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+template <int N>
+__device__ __forceinline__ void nbh_softmax_add(nbh_softmax &s, const float (&f)[N], float scale)
+{
+    float peak = f[0];
+    for (int i = 1; i < N; ++i)
+        peak = fmaxf(peak, f[i]);
+    peak = fmaxf(s.peak, fminf(peak, FLT_MAX));
+    float sum[2] = {0.0f, 0.0f};
+    for (int i = 0; i < N; i += 2) {
+        sum[0] += nbh_exp2((f[i] - peak) * scale);
+        sum[1] += nbh_exp2((f[i + 1] - peak) * scale);
+    }
+    s.sum = s.sum * nbh_exp2((s.peak - peak) * scale) + (sum[0] + sum[1]);
+    s.peak = peak;
+}
+__device__ __forceinline__ nbh_softmax nbh_softmax_join(nbh_softmax a, nbh_softmax b, float scale)
+{
+    const float peak = fmaxf(a.peak, b.peak);
+    return {peak, a.sum * nbh_exp2((a.peak - peak) * scale) + b.sum * nbh_exp2((b.peak - peak) * scale)};
+}
+// log sum exp(x / temperature)
+__device__ __forceinline__ float nbh_softmax_lse(nbh_softmax s, float temperature)
+{
+    return s.peak / temperature + logf(s.sum);
+}
+// Over a workgroup of `T` lanes; `room` holds T / 64 entries.  Every lane gets the result.
+template <int T>
+__device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float scale, nbh_softmax *room)
+{
+    for (int step = 32; step; step >>= 1) {
+        const nbh_softmax other = {__shfl_xor(s.peak, step), __shfl_xor(s.sum, step)};
+        s = nbh_softmax_join(s, other, scale);
+    }
+    if ((threadIdx.x & 63) == 0)
+        room[threadIdx.x >> 6] = s;
+    __syncthreads();
+    s = room[0];
+    for (int w = 1; w < T / 64; ++w)
+        s = nbh_softmax_join(s, room[w], scale);
+    return s;
+}
+
+// Temperatures whose reciprocal is an ordinary float32 number.
+static inline bool nbh_row_temperature(double t) { return t >= 1e-30 && t <= 1e30; }
+
+// 4- or 8-byte integers, as the caller's arrays hold them.
+__device__ __forceinline__ int64_t nbh_row_int(const void *p, int bytes, int64_t at)
+{
+    return bytes == 8 ? static_cast<const int64_t *>(p)[at] : static_cast<const int32_t *>(p)[at];
+}
+__device__ __forceinline__ int64_t nbh_row_clamp(int64_t x, int64_t low, int64_t high)
+{
+    return x < low ? low : x > high ? high : x;
+}

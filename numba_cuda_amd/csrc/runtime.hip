@@ -178,6 +178,16 @@ int nbh_mem_address_range(void **base, size_t *size, void *dptr)
     return 0;
 }
 
+int nbh_pointer_device(const void *address, int *dev)
+{
+    if (!dev)
+        return (int)hipErrorInvalidValue;
+    hipPointerAttribute_t attributes;
+    NBH_TRY(hipPointerGetAttributes(&attributes, address));
+    *dev = attributes.device;
+    return 0;
+}
+
 // ---- sharing an allocation with another process ---------------------------------------
 // Handles are hipIpcMemHandle_t, 64 opaque bytes.  Opening an allocation of 2 GiB or more
 // has been seen not to return on MI355X hosts, so such allocations are refused on both
@@ -311,6 +321,16 @@ int nbh_stream_synchronize(nbh_stream_t stream)
     return rc ? rc : queued;
 }
 int nbh_stream_query(nbh_stream_t stream) { return (int)hipStreamQuery(nbh_hip_stream(stream)); }
+
+int nbh_stream_is_capturing(nbh_stream_t stream, int *capturing)
+{
+    if (!capturing)
+        return (int)hipErrorInvalidValue;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    NBH_TRY(hipStreamIsCapturing((hipStream_t)stream, &status));
+    *capturing = status != hipStreamCaptureStatusNone;
+    return 0;
+}
 
 int nbh_stream_add_callback(nbh_stream_t stream, nbh_host_fn fn, void *user)
 {

@@ -757,6 +757,7 @@ class Context:
         self._scratch_lock = threading.Lock()
         self._scratch = {}          # stream handle -> (address, bytes, memory) of nbh_reduce's scratch
         self._scratch_tls = threading.local()   # the same for each thread's per-thread default stream
+        self._workspaces = {}       # stream handle -> (address, bytes, memory) for the row operators
         self._result_cells = _ResultCells()
 
     @property
@@ -773,6 +774,7 @@ class Context:
         _logger.info("reset context of device %s", self.device.id)
         with self._scratch_lock:
             self._scratch.clear()
+            self._workspaces.clear()
         self._scratch_tls = threading.local()
         self._result_cells.release_all()
         self._memory_manager.reset()
@@ -906,10 +908,34 @@ class Context:
         driver.nbh_memset8(address, 0, nbytes, None)
         return address, nbytes, mem
 
+    def workspace(self, stream_handle, nbytes):
+        """(address, size, memory) of at least `nbytes` bytes for the row operators on the given
+        stream (kernels/logits.py), kept and grown as calls need it.  Whoever launches work
+        that uses it holds on to the memory until the launch is made: another thread may
+        replace the entry meanwhile.  Kept per thread for the per-thread default stream."""
+        if stream_handle == HIP_STREAM_PER_THREAD:
+            entry = getattr(self._scratch_tls, "workspace", None)
+            if entry is None or entry[1] < nbytes:
+                entry = self._scratch_tls.workspace = self._new_workspace(nbytes)
+            return entry
+        entry = self._workspaces.get(stream_handle)
+        if entry is None or entry[1] < nbytes:
+            with self._scratch_lock:
+                entry = self._workspaces.get(stream_handle)
+                if entry is None or entry[1] < nbytes:
+                    entry = self._workspaces[stream_handle] = self._new_workspace(nbytes)
+        return entry
+
+    def _new_workspace(self, nbytes):
+        nbytes = max(1 << 20, 1 << (nbytes - 1).bit_length())
+        mem = self.memalloc(nbytes)
+        return mem.device_ctypes_pointer.value, nbytes, mem
+
     def _forget_stream(self, stream_handle):
         """The stream is about to be destroyed: let go of what was kept for it."""
         with self._scratch_lock:
             self._scratch.pop(stream_handle, None)
+            self._workspaces.pop(stream_handle, None)
 
     def take_result_cell(self):
         """(device address, 16 host bytes as a uint8 array) for one result; hand it

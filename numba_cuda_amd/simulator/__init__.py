@@ -10,7 +10,7 @@ the RNG runs on host state arrays.  No GPU library is loaded in this mode.
 from numba_cuda_amd.core.errors import CudaDriverError, CudaSupportError, NumbaPerformanceWarning  # noqa: F401
 from numba_cuda_amd.simulator.args import In, InOut, Out  # noqa: F401
 from numba_cuda_amd.simulator import hostarray as devicearray  # noqa: F401
-from numba_cuda_amd.simulator import random, reduction  # noqa: F401
+from numba_cuda_amd.simulator import logits, random, reduction  # noqa: F401
 from numba_cuda_amd.simulator.hostarray import (HostBackedArray, DeviceNDArray, DeviceRecord,  # noqa: F401
                                                 _contiguous_strides_like_array, _order_like_array, auto_device,
                                                 device_array, device_array_like, is_cuda_ndarray, managed_array,
