@@ -6,17 +6,19 @@
 //   x' = x' + bias(v)                      the last pair of the row that names v
 //   out = v allowed by the mask ? x' : -inf
 //
-// A workgroup owns a tile of one row's vocabulary.  It counts the row's history into one LDS word per
-// entry (bit 31: seen, below it the count) and notes the bias pairs that fall into the tile, each token
-// of the history read by every tile of the row (from L2), then streams the tile once: 16 bytes per lane,
-// one or two LDS reads for what the tile knows about them.  Integer LDS atomics only: the order in which
-// lanes arrive changes nothing.
+// A workgroup owns a tile of one row's vocabulary.  It asks for the tile's logits and mask first and
+// counts the row's history into one LDS word per entry (below) while they are on their way; every tile of
+// a row reads the whole history, from L2.  Bias pairs of the tile go to a short list.  Integer LDS atomics
+// only, and of the pairs the one with the largest number counts: the order in which lanes arrive changes
+// nothing.
 #include "rows.h"
 
 namespace {
 
-constexpr uint32_t kSeen = 0x80000000u;
-constexpr int kTile = 4096;
+// The word of an entry: bit 31 it occurs in the history, bit 30 a pair of the list names it, below them
+// how often it occurs behind the prompt.
+constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffffffu;
+constexpr int kPairs = 256;              // bias pairs a tile lists; the rest of them are looked up in memory
 
 struct Adjust {
     const char *in;
@@ -36,64 +38,111 @@ struct Adjust {
     int64_t mask_stride;
 };
 
-// One entry, everything but the mask.
-__device__ __forceinline__ float adjusted(float x, uint32_t word, float bias, bool biased, float repetition,
-                                          float presence, float frequency)
+// Integers of 4 or 8 bytes p[begin .. end), 16 bytes per lane and load, four loads on their way at a time:
+// visit(v) for every v in [first, first + n), less `first`.
+template <int T, typename I, typename F>
+__device__ __forceinline__ void visit_tokens(const I *p, int64_t begin, int64_t end, int64_t first, uint32_t n, F visit)
 {
-    if (word) {
-        x = x > 0.0f ? x / repetition : x * repetition;
-        const uint32_t count = word & ~kSeen;
-        if (count) {
-            x = x - frequency * (float)count;
-            x = x - presence;
+    constexpr int kEach = 16 / sizeof(I), kAhead = 4;
+    int64_t at = begin + threadIdx.x * kEach;
+    for (; at + (kAhead - 1) * T * kEach + kEach <= end; at += kAhead * T * kEach) {
+        nbh_u32x4 v[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            v[j] = nbh_load16<sizeof(I), false>(p + at + j * T * kEach);
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) {
+                if constexpr (sizeof(I) == 4) {
+                    const uint32_t t = (uint32_t)v[j][i] - (uint32_t)first;
+                    if (t < n)
+                        visit(t);
+                } else {
+                    const uint64_t t = ((uint64_t)v[j][2 * i + 1] << 32 | v[j][2 * i]) - (uint64_t)first;
+                    if (t < n)
+                        visit((uint32_t)t);
+                }
+            }
+    }
+    for (; at < end; at += T * kEach) {
+        I v[kEach];
+        if (at + kEach <= end)
+            __builtin_memcpy(v, p + at, 16);
+        else
+            for (int i = 0; i < kEach; ++i)
+                v[i] = at + i < end ? p[at + i] : -1;
+        for (int i = 0; i < kEach; ++i) {
+            const uint64_t t = (uint64_t)((int64_t)v[i] - first);
+            if (v[i] >= 0 && t < n)
+                visit((uint32_t)t);
         }
     }
-    return biased ? x + bias : x;
+}
+template <int T, typename F>
+__device__ __forceinline__ void visit_tokens(const void *p, int bytes, int64_t begin, int64_t end, int64_t first,
+                                             uint32_t n, F visit)
+{
+    if (bytes == 4)
+        visit_tokens<T>(static_cast<const int32_t *>(p), begin, end, first, n, visit);
+    else
+        visit_tokens<T>(static_cast<const int64_t *>(p), begin, end, first, n, visit);
 }
 
-template <typename In, typename Out, int T>
+template <typename In, typename Out, int T, int TILE>
 __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
 {
-    extern __shared__ uint32_t words[];              // kTile words, then kTile pair numbers if there are biases
-    constexpr int kItems = In::items;
+    constexpr int kItems = In::items, kVecs = TILE / (T * kItems);
+    __shared__ uint32_t words[TILE];
+    __shared__ uint32_t pair_at[kPairs], pair_number[kPairs];
+    __shared__ uint32_t pair_count;
     const int64_t row = a.row0 + blockIdx.x / a.tiles;
     const int tile = blockIdx.x % a.tiles;
-    const int64_t first = (int64_t)tile * kTile;
-    const int n = (int)(a.vocab - first < kTile ? a.vocab - first : kTile);
-    uint32_t *const pairs = words + kTile;
+    const int64_t first = (int64_t)tile * TILE;
+    const int n = (int)(a.vocab - first < TILE ? a.vocab - first : TILE);
+
+    const typename In::item *in = reinterpret_cast<const typename In::item *>(a.in + row * a.in_stride) + first;
+    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + first / 8 : nullptr;
+    nbh_u32x4 raw[kVecs];
+    uint32_t bits[kVecs];
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+        const int at = (j * T + threadIdx.x) * kItems;
+        raw[j] = nbh_row_load_raw<In, true>(in, at, n, 0);
+        // bits of these entries, the first the lowest; a mask row ends with its last entry's word
+        bits[j] = mask && at < n ? (uint32_t)mask[at / 8] >> (at & 7) : 0xffu;
+    }
 
     const bool history = a.tokens != nullptr, biases = a.bias_tokens != nullptr;
-    if (history)
-        for (int i = threadIdx.x * 4; i < kTile; i += T * 4)
+    int64_t pair0 = 0, pair1 = 0;
+    if (history || biases) {
+        for (int i = threadIdx.x * 4; i < TILE; i += T * 4)
             *reinterpret_cast<uint4 *>(words + i) = uint4{0, 0, 0, 0};
-    if (biases)
-        for (int i = threadIdx.x * 4; i < kTile; i += T * 4)
-            *reinterpret_cast<uint4 *>(pairs + i) = uint4{0, 0, 0, 0};
-    if (history || biases)
+        if (threadIdx.x == 0)
+            pair_count = 0;
         __syncthreads();
+    }
     if (history) {
         const int64_t begin = nbh_row_clamp(nbh_row_int(a.offsets, a.offset_bytes, row), 0, a.n_tokens);
         const int64_t end = nbh_row_clamp(nbh_row_int(a.offsets, a.offset_bytes, row + 1), begin, a.n_tokens);
         const int64_t made =
             a.prompts ? begin + nbh_row_clamp(nbh_row_int(a.prompts, a.prompt_bytes, row), 0, end - begin) : begin;
-        for (int64_t i = begin + threadIdx.x; i < end; i += T) {
-            const int64_t at = nbh_row_int(a.tokens, a.token_bytes, i) - first;
-            if (at >= 0 && at < n) {
-                if (i >= made)
-                    atomicAdd(&words[at], 1u);
-                else
-                    atomicOr(&words[at], kSeen);
-            }
-        }
+        visit_tokens<T>(a.tokens, a.token_bytes, begin, made, first, n, [&](uint32_t t) { atomicOr(&words[t], kSeen); });
+        visit_tokens<T>(a.tokens, a.token_bytes, made, end, first, n, [&](uint32_t t) { atomicAdd(&words[t], 1u); });
     }
-    int64_t pair0 = 0;
     if (biases) {
         pair0 = nbh_row_clamp(nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row), 0, a.n_bias);
-        const int64_t end = nbh_row_clamp(nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row + 1), pair0, a.n_bias);
-        for (int64_t i = pair0 + threadIdx.x; i < end; i += T) {
+        pair1 = nbh_row_clamp(nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row + 1), pair0, a.n_bias);
+        for (int64_t i = pair0 + threadIdx.x; i < pair1; i += T) {
             const int64_t at = nbh_row_int(a.bias_tokens, a.bias_token_bytes, i) - first;
-            if (at >= 0 && at < n)
-                atomicMax(&pairs[at], (uint32_t)(i - pair0 + 1));
+            if (at >= 0 && at < n) {
+                atomicOr(&words[at], kBiased);
+                const uint32_t place = atomicAdd(&pair_count, 1u);
+                if (place < kPairs) {
+                    pair_at[place] = (uint32_t)at;
+                    pair_number[place] = (uint32_t)(i - pair0);
+                }
+            }
         }
     }
     if (history || biases)
@@ -102,27 +151,51 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
     const float repetition = a.repetition ? a.repetition[row] : a.repetition_value;
     const float presence = a.presence ? a.presence[row] : a.presence_value;
     const float frequency = a.frequency ? a.frequency[row] : a.frequency_value;
-    const typename In::item *in = reinterpret_cast<const typename In::item *>(a.in + row * a.in_stride) + first;
     typename Out::item *out = reinterpret_cast<typename Out::item *>(a.out + row * a.out_stride) + first;
-    const uint8_t *mask = a.mask ? a.mask + row * a.mask_stride + first / 8 : nullptr;
 
-    for (int at = threadIdx.x * kItems; at < n; at += T * kItems) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+        const int at = (j * T + threadIdx.x) * kItems;
+        if (at >= n)
+            break;
         float f[kItems];
-        nbh_row_load<In, true>(in, at, n, 0.0f, f);
-        // bits of these entries, the first the lowest; a mask row ends with its last entry's word
-        const uint32_t bits = mask ? (uint32_t)mask[at / 8] >> (at & 7) : 0xffu;
-        uint32_t word[kItems], pair[kItems], any = 0;
-        for (int i = 0; i < kItems; ++i) {
-            word[i] = history ? words[at + i] : 0u;
-            pair[i] = biases ? pairs[at + i] : 0u;
-            any |= word[i] | pair[i];
+        In::unpack(raw[j], f);
+        if (history || biases) {
+            uint32_t word[kItems], any = 0;
+            for (int i = 0; i < kItems; ++i) {
+                word[i] = words[at + i];
+                any |= word[i];
+            }
+            if (any)
+                for (int i = 0; i < kItems; ++i) {
+                    if (!word[i])
+                        continue;
+                    const uint32_t count = word[i] & kCount;
+                    float x = f[i];
+                    if (word[i] & kSeen || count)
+                        x = x > 0.0f ? x / repetition : x * repetition;
+                    if (count) {
+                        x = x - frequency * (float)count;
+                        x = x - presence;
+                    }
+                    if (word[i] & kBiased) {
+                        int64_t last = -1;
+                        if (pair_count <= kPairs) {
+                            for (uint32_t k = 0; k < pair_count; ++k)
+                                if (pair_at[k] == (uint32_t)(at + i) && (int64_t)pair_number[k] > last)
+                                    last = pair_number[k];
+                        } else {
+                            for (int64_t k = pair1 - pair0; last < 0 && k-- > 0;)
+                                if (nbh_row_int(a.bias_tokens, a.bias_token_bytes, pair0 + k) == first + at + i)
+                                    last = k;
+                        }
+                        x = x + a.bias_values[pair0 + last];
+                    }
+                    f[i] = x;
+                }
         }
-        if (any)
-            for (int i = 0; i < kItems; ++i)
-                f[i] = adjusted(f[i], word[i], pair[i] ? a.bias_values[pair0 + pair[i] - 1] : 0.0f, pair[i] != 0,
-                                repetition, presence, frequency);
         for (int i = 0; i < kItems; ++i)
-            f[i] = bits >> i & 1u ? f[i] : -INFINITY;
+            f[i] = bits[j] >> i & 1u ? f[i] : -INFINITY;
         if constexpr (Out::items == kItems) {
             nbh_row_store<Out, true>(out, at, n, f);
         } else {
@@ -136,21 +209,27 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
     }
 }
 
-template <typename In, typename Out>
+template <typename In, typename Out, int T, int TILE>
 int launch_adjust(Adjust a, int64_t rows, hipStream_t stream)
 {
-    const size_t lds = (size_t)kTile * 4 * ((a.tokens ? 1 : 0) + (a.bias_tokens ? 1 : 0));
-    // the pair numbers follow the words in any case
-    const size_t bytes = a.bias_tokens ? (size_t)kTile * 8 : lds;
+    a.tiles = (int)((a.vocab + TILE - 1) / TILE);
     // a launch holds less than 2^32 lanes
     const int64_t most = NBH_ROW_MOST_GROUPS / a.tiles;
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t groups = (rows - a.row0 < most ? rows - a.row0 : most) * a.tiles;
-        adjust_rows<In, Out, 256><<<dim3((unsigned)groups), dim3(256), bytes, stream>>>(a);
+        adjust_rows<In, Out, T, TILE><<<dim3((unsigned)groups), dim3(T), 0, stream>>>(a);
         if (const int status = nbh_launch_status())
             return status;
     }
     return 0;
+}
+template <typename In, typename Out>
+int launch_adjust(const Adjust &a, int64_t rows, hipStream_t stream)
+{
+    // Long histories cost more than the row: fewer, larger workgroups read them less often.
+    if (a.n_tokens / rows > 8192)
+        return launch_adjust<In, Out, 1024, 16384>(a, rows, stream);
+    return launch_adjust<In, Out, 256, 4096>(a, rows, stream);
 }
 
 }  // namespace
@@ -163,7 +242,7 @@ extern "C" int nbh_logits_adjust(const struct nbh_logits_adjust_args *p, nbh_str
         return 0;
     const bool same = p->out_dtype == p->dtype;
     if (!p->logits || !p->out || p->dtype < 0 || p->dtype > NBH_ROW_BF16 || !(same || p->out_dtype == NBH_ROW_F32) ||
-        p->vocab > INT32_MAX || p->n_tokens < 0 || p->n_tokens > INT32_MAX || p->n_bias < 0 || p->n_bias > INT32_MAX)
+        p->vocab > INT32_MAX || p->n_tokens < 0 || p->n_tokens >= (1 << 30) || p->n_bias < 0 || p->n_bias > INT32_MAX)
         return (int)hipErrorInvalidValue;
     auto width = [](int64_t b) { return b == 4 || b == 8; };
     const bool history = p->tokens && p->n_tokens, biases = p->bias_tokens && p->n_bias;
@@ -178,7 +257,6 @@ extern "C" int nbh_logits_adjust(const struct nbh_logits_adjust_args *p, nbh_str
     a.in_stride = p->in_stride;
     a.out_stride = p->out_stride;
     a.vocab = p->vocab;
-    a.tiles = (int)((p->vocab + kTile - 1) / kTile);
     if (history) {
         a.tokens = p->tokens;
         a.offsets = p->offsets;

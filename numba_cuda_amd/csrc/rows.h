@@ -21,6 +21,8 @@ typedef __bf16 nbh_bf16x2 __attribute__((ext_vector_type(2)));
 struct nbh_row_f32 {
     typedef float item;
     static constexpr int items = 4;
+    static constexpr uint32_t lowest = 0xff800000u;      // bits of -inf
+    static __device__ __forceinline__ uint32_t bits(item x) { return __float_as_uint(x); }
     static __device__ __forceinline__ float get(item x) { return x; }
     static __device__ __forceinline__ item put(float x) { return x; }
     static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[4])
@@ -39,6 +41,8 @@ struct nbh_row_f32 {
 struct nbh_row_f16 {
     typedef _Float16 item;
     static constexpr int items = 8;
+    static constexpr uint32_t lowest = 0xfc00u;
+    static __device__ __forceinline__ uint32_t bits(item x) { return __builtin_bit_cast(uint16_t, x); }
     static __device__ __forceinline__ float get(item x) { return (float)x; }
     static __device__ __forceinline__ item put(float x) { return (item)x; }
     static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[8])
@@ -62,6 +66,8 @@ struct nbh_row_f16 {
 struct nbh_row_bf16 {
     typedef uint16_t item;
     static constexpr int items = 8;
+    static constexpr uint32_t lowest = 0xff80u;
+    static __device__ __forceinline__ uint32_t bits(item x) { return x; }
     static __device__ __forceinline__ float get(item x) { return __uint_as_float((uint32_t)x << 16); }
     static __device__ __forceinline__ item put(float x)
     {
@@ -85,7 +91,23 @@ struct nbh_row_bf16 {
     }
 };
 
-// The 16 bytes at element `at` of a row of `n` elements; elements behind the row's end read as `fill`.
+// The 16 bytes at element `at` of a row of `n` elements; elements behind the row's end read as `fill`, the
+// raw one as its bits.
+template <typename E, bool NT>
+__device__ __forceinline__ nbh_u32x4 nbh_row_load_raw(const typename E::item *row, int64_t at, int64_t n, uint32_t fill)
+{
+    if (at + E::items <= n)
+        return nbh_load16<sizeof(typename E::item), NT>(row + at);
+    nbh_u32x4 v = {};
+    for (int i = 0; i < E::items; ++i) {
+        const uint32_t bits = at + i < n ? E::bits(row[at + i]) : fill;
+        if (E::items == 4)
+            v[i] = bits;
+        else
+            v[i / 2] |= bits << (i % 2 * 16);
+    }
+    return v;
+}
 template <typename E, bool NT>
 __device__ __forceinline__ void nbh_row_load(const typename E::item *row, int64_t at, int64_t n, float fill,
                                              float (&f)[E::items])
