@@ -38,44 +38,45 @@ struct Adjust {
     int64_t mask_stride;
 };
 
-// Integers of 4 or 8 bytes p[begin .. end), 16 bytes per lane and load, four loads on their way at a time:
-// visit(v) for every v in [first, first + n), less `first`.
+// The integers p[0 .. count), 16 bytes per lane and load, four loads on their way at a time:
+// visit(v - first, number) for every v in [first, first + n).
 template <int T, typename I, typename F>
-__device__ __forceinline__ void visit_tokens(const I *p, int64_t begin, int64_t end, int64_t first, uint32_t n, F visit)
+__device__ __forceinline__ void visit_tokens(const I *p, int count, int64_t first, uint32_t n, F visit)
 {
     constexpr int kEach = 16 / sizeof(I), kAhead = 4;
-    int64_t at = begin + threadIdx.x * kEach;
-    for (; at + (kAhead - 1) * T * kEach + kEach <= end; at += kAhead * T * kEach) {
+    auto use = [&](nbh_u32x4 v, int at) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if constexpr (sizeof(I) == 4) {
+                const uint32_t t = v[i] - (uint32_t)first;
+                if (t < n)
+                    visit(t, at + i);
+            } else {
+                const uint64_t t = ((uint64_t)v[2 * i + 1] << 32 | v[2 * i]) - (uint64_t)first;
+                if (t < n)
+                    visit((uint32_t)t, at + i);
+            }
+        }
+    };
+    int base = 0;                        // of the workgroup
+    for (; base + kAhead * T * kEach <= count; base += kAhead * T * kEach) {
         nbh_u32x4 v[kAhead];
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
-            v[j] = nbh_load16<sizeof(I), false>(p + at + j * T * kEach);
+            v[j] = nbh_load16<sizeof(I), false>(p + base + (j * T + threadIdx.x) * kEach);
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
-#pragma unroll
-            for (int i = 0; i < kEach; ++i) {
-                if constexpr (sizeof(I) == 4) {
-                    const uint32_t t = (uint32_t)v[j][i] - (uint32_t)first;
-                    if (t < n)
-                        visit(t);
-                } else {
-                    const uint64_t t = ((uint64_t)v[j][2 * i + 1] << 32 | v[j][2 * i]) - (uint64_t)first;
-                    if (t < n)
-                        visit((uint32_t)t);
-                }
-            }
+            use(v[j], base + (j * T + threadIdx.x) * kEach);
     }
-    for (; at < end; at += T * kEach) {
-        I v[kEach];
-        if (at + kEach <= end)
-            __builtin_memcpy(v, p + at, 16);
-        else
-            for (int i = 0; i < kEach; ++i)
-                v[i] = at + i < end ? p[at + i] : -1;
-        for (int i = 0; i < kEach; ++i) {
-            const uint64_t t = (uint64_t)((int64_t)v[i] - first);
-            if (v[i] >= 0 && t < n)
-                visit((uint32_t)t);
+    for (int at = base + threadIdx.x * kEach; at < count; at += T * kEach) {
+        if (at + kEach <= count) {
+            use(nbh_load16<sizeof(I), false>(p + at), at);
+        } else {
+            for (int i = at; i < count; ++i) {
+                const uint64_t t = (uint64_t)((int64_t)p[i] - first);
+                if (t < n)
+                    visit((uint32_t)t, i);
+            }
         }
     }
 }
@@ -84,15 +85,16 @@ __device__ __forceinline__ void visit_tokens(const void *p, int bytes, int64_t b
                                              uint32_t n, F visit)
 {
     if (bytes == 4)
-        visit_tokens<T>(static_cast<const int32_t *>(p), begin, end, first, n, visit);
+        visit_tokens<T>(static_cast<const int32_t *>(p) + begin, (int)(end - begin), first, n, visit);
     else
-        visit_tokens<T>(static_cast<const int64_t *>(p), begin, end, first, n, visit);
+        visit_tokens<T>(static_cast<const int64_t *>(p) + begin, (int)(end - begin), first, n, visit);
 }
 
 template <typename In, typename Out, int T, int TILE>
 __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
 {
     constexpr int kItems = In::items, kVecs = TILE / (T * kItems);
+    static_assert(Out::items == kItems, "as many entries per vector on both sides");
     __shared__ uint32_t words[TILE];
     __shared__ uint32_t pair_at[kPairs], pair_number[kPairs];
     __shared__ uint32_t pair_count;
@@ -108,13 +110,26 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
         const int at = (j * T + threadIdx.x) * kItems;
-        raw[j] = nbh_row_load_raw<In, true>(in, at, n, 0);
+        raw[j] = nbh_row_load_raw<In, false>(in, at, n, 0);
         // bits of these entries, the first the lowest; a mask row ends with its last entry's word
         bits[j] = mask && at < n ? (uint32_t)mask[at / 8] >> (at & 7) : 0xffu;
     }
 
+    // everything about the row, asked for at once
     const bool history = a.tokens != nullptr, biases = a.bias_tokens != nullptr;
-    int64_t pair0 = 0, pair1 = 0;
+    int64_t begin = 0, end = 0, prompt_length = 0, pair0 = 0, pair1 = 0;
+    if (history) {
+        begin = nbh_row_int(a.offsets, a.offset_bytes, row);
+        end = nbh_row_int(a.offsets, a.offset_bytes, row + 1);
+        prompt_length = a.prompts ? nbh_row_int(a.prompts, a.prompt_bytes, row) : 0;
+    }
+    if (biases) {
+        pair0 = nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row);
+        pair1 = nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row + 1);
+    }
+    const float repetition = a.repetition ? a.repetition[row] : a.repetition_value;
+    const float presence = a.presence ? a.presence[row] : a.presence_value;
+    const float frequency = a.frequency ? a.frequency[row] : a.frequency_value;
     if (history || biases) {
         for (int i = threadIdx.x * 4; i < TILE; i += T * 4)
             *reinterpret_cast<uint4 *>(words + i) = uint4{0, 0, 0, 0};
@@ -123,34 +138,31 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
         __syncthreads();
     }
     if (history) {
-        const int64_t begin = nbh_row_clamp(nbh_row_int(a.offsets, a.offset_bytes, row), 0, a.n_tokens);
-        const int64_t end = nbh_row_clamp(nbh_row_int(a.offsets, a.offset_bytes, row + 1), begin, a.n_tokens);
-        const int64_t made =
-            a.prompts ? begin + nbh_row_clamp(nbh_row_int(a.prompts, a.prompt_bytes, row), 0, end - begin) : begin;
-        visit_tokens<T>(a.tokens, a.token_bytes, begin, made, first, n, [&](uint32_t t) { atomicOr(&words[t], kSeen); });
-        visit_tokens<T>(a.tokens, a.token_bytes, made, end, first, n, [&](uint32_t t) { atomicAdd(&words[t], 1u); });
+        begin = nbh_row_clamp(begin, 0, a.n_tokens);
+        end = nbh_row_clamp(end, begin, a.n_tokens);
+        const int prompt = (int)nbh_row_clamp(prompt_length, 0, end - begin);
+        visit_tokens<T>(a.tokens, a.token_bytes, begin, end, first, n, [&](uint32_t t, int i) {
+            if (i < prompt)
+                atomicOr(&words[t], kSeen);
+            else
+                atomicAdd(&words[t], 1u);
+        });
     }
     if (biases) {
-        pair0 = nbh_row_clamp(nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row), 0, a.n_bias);
-        pair1 = nbh_row_clamp(nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row + 1), pair0, a.n_bias);
-        for (int64_t i = pair0 + threadIdx.x; i < pair1; i += T) {
-            const int64_t at = nbh_row_int(a.bias_tokens, a.bias_token_bytes, i) - first;
-            if (at >= 0 && at < n) {
-                atomicOr(&words[at], kBiased);
-                const uint32_t place = atomicAdd(&pair_count, 1u);
-                if (place < kPairs) {
-                    pair_at[place] = (uint32_t)at;
-                    pair_number[place] = (uint32_t)(i - pair0);
-                }
+        pair0 = nbh_row_clamp(pair0, 0, a.n_bias);
+        pair1 = nbh_row_clamp(pair1, pair0, a.n_bias);
+        visit_tokens<T>(a.bias_tokens, a.bias_token_bytes, pair0, pair1, first, n, [&](uint32_t t, int i) {
+            atomicOr(&words[t], kBiased);
+            const uint32_t place = atomicAdd(&pair_count, 1u);
+            if (place < kPairs) {
+                pair_at[place] = t;
+                pair_number[place] = (uint32_t)i;
             }
-        }
+        });
     }
     if (history || biases)
         __syncthreads();
 
-    const float repetition = a.repetition ? a.repetition[row] : a.repetition_value;
-    const float presence = a.presence ? a.presence[row] : a.presence_value;
-    const float frequency = a.frequency ? a.frequency[row] : a.frequency_value;
     typename Out::item *out = reinterpret_cast<typename Out::item *>(a.out + row * a.out_stride) + first;
 
 #pragma unroll
@@ -196,16 +208,7 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
         }
         for (int i = 0; i < kItems; ++i)
             f[i] = bits[j] >> i & 1u ? f[i] : -INFINITY;
-        if constexpr (Out::items == kItems) {
-            nbh_row_store<Out, true>(out, at, n, f);
-        } else {
-            for (int h = 0; h < kItems; h += Out::items) {
-                float part[Out::items];
-                for (int i = 0; i < Out::items; ++i)
-                    part[i] = f[h + i];
-                nbh_row_store<Out, true>(out, at + h, n, part);
-            }
-        }
+        nbh_row_store<Out, true>(out, at, n, f);
     }
 }
 
@@ -228,7 +231,7 @@ int launch_adjust(const Adjust &a, int64_t rows, hipStream_t stream)
 {
     // Long histories cost more than the row: fewer, larger workgroups read them less often.
     if (a.n_tokens / rows > 8192)
-        return launch_adjust<In, Out, 1024, 16384>(a, rows, stream);
+        return launch_adjust<In, Out, 1024, 8192>(a, rows, stream);
     return launch_adjust<In, Out, 256, 4096>(a, rows, stream);
 }
 
@@ -290,9 +293,9 @@ extern "C" int nbh_logits_adjust(const struct nbh_logits_adjust_args *p, nbh_str
         return launch_adjust<nbh_row_f32, nbh_row_f32>(a, p->rows, s);
     case NBH_ROW_F16:
         return same ? launch_adjust<nbh_row_f16, nbh_row_f16>(a, p->rows, s)
-                    : launch_adjust<nbh_row_f16, nbh_row_f32>(a, p->rows, s);
+                    : launch_adjust<nbh_row_half<nbh_row_f16>, nbh_row_f32>(a, p->rows, s);
     default:
         return same ? launch_adjust<nbh_row_bf16, nbh_row_bf16>(a, p->rows, s)
-                    : launch_adjust<nbh_row_bf16, nbh_row_f32>(a, p->rows, s);
+                    : launch_adjust<nbh_row_half<nbh_row_bf16>, nbh_row_f32>(a, p->rows, s);
     }
 }

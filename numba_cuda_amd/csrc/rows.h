@@ -22,6 +22,7 @@ struct nbh_row_f32 {
     typedef float item;
     static constexpr int items = 4;
     static constexpr uint32_t lowest = 0xff800000u;      // bits of -inf
+    template <bool NT> static __device__ __forceinline__ nbh_u32x4 load(const item *p) { return nbh_load16<4, NT>(p); }
     static __device__ __forceinline__ uint32_t bits(item x) { return __float_as_uint(x); }
     static __device__ __forceinline__ float get(item x) { return x; }
     static __device__ __forceinline__ item put(float x) { return x; }
@@ -42,6 +43,7 @@ struct nbh_row_f16 {
     typedef _Float16 item;
     static constexpr int items = 8;
     static constexpr uint32_t lowest = 0xfc00u;
+    template <bool NT> static __device__ __forceinline__ nbh_u32x4 load(const item *p) { return nbh_load16<2, NT>(p); }
     static __device__ __forceinline__ uint32_t bits(item x) { return __builtin_bit_cast(uint16_t, x); }
     static __device__ __forceinline__ float get(item x) { return (float)x; }
     static __device__ __forceinline__ item put(float x) { return (item)x; }
@@ -67,6 +69,7 @@ struct nbh_row_bf16 {
     typedef uint16_t item;
     static constexpr int items = 8;
     static constexpr uint32_t lowest = 0xff80u;
+    template <bool NT> static __device__ __forceinline__ nbh_u32x4 load(const item *p) { return nbh_load16<2, NT>(p); }
     static __device__ __forceinline__ uint32_t bits(item x) { return x; }
     static __device__ __forceinline__ float get(item x) { return __uint_as_float((uint32_t)x << 16); }
     static __device__ __forceinline__ item put(float x)
@@ -91,17 +94,40 @@ struct nbh_row_bf16 {
     }
 };
 
+// The two-byte types four at a time, for results of four bytes: a wavefront's stores are then whole lines.
+typedef uint32_t nbh_u32x2 __attribute__((ext_vector_type(2)));
+typedef nbh_u32x2 nbh_u32x2_any __attribute__((aligned(2)));
+template <typename E> struct nbh_row_half {
+    typedef typename E::item item;
+    static constexpr int items = 4;
+    static constexpr uint32_t lowest = E::lowest;
+    template <bool NT> static __device__ __forceinline__ nbh_u32x4 load(const item *p)
+    {
+        const nbh_u32x2_any *q = reinterpret_cast<const nbh_u32x2_any *>(p);
+        const nbh_u32x2 v = NT ? __builtin_nontemporal_load(q) : *q;
+        return nbh_u32x4{v[0], v[1], 0, 0};
+    }
+    static __device__ __forceinline__ uint32_t bits(item x) { return E::bits(x); }
+    static __device__ __forceinline__ void unpack(nbh_u32x4 v, float (&f)[4])
+    {
+        float all[8];
+        E::unpack(v, all);
+        for (int i = 0; i < 4; ++i)
+            f[i] = all[i];
+    }
+};
+
 // The 16 bytes at element `at` of a row of `n` elements; elements behind the row's end read as `fill`, the
 // raw one as its bits.
 template <typename E, bool NT>
 __device__ __forceinline__ nbh_u32x4 nbh_row_load_raw(const typename E::item *row, int64_t at, int64_t n, uint32_t fill)
 {
     if (at + E::items <= n)
-        return nbh_load16<sizeof(typename E::item), NT>(row + at);
+        return E::template load<NT>(row + at);
     nbh_u32x4 v = {};
     for (int i = 0; i < E::items; ++i) {
         const uint32_t bits = at + i < n ? E::bits(row[at + i]) : fill;
-        if (E::items == 4)
+        if (sizeof(typename E::item) == 4)
             v[i] = bits;
         else
             v[i / 2] |= bits << (i % 2 * 16);
