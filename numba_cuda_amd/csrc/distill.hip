@@ -15,7 +15,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
-constexpr int kVecs = 4;
+constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f;       // log2(e) and its rounding
+constexpr float kLn2 = 0.693147180559945309f;
 
 struct Distill {
     const char *student;
@@ -26,28 +27,13 @@ struct Distill {
     const float *teacher_lse, *grad_loss;
     int64_t grad_loss_stride;
     float grad_loss_value;
-    float temperature, scale;            // scale = log2(e) / temperature
+    float temperature, scale, scale_rest;    // log2(e) / temperature, and what its rounding took off
     float *loss, *lse;
     char *grad;
     int64_t grad_stride;
     nbh_softmax *parts;                  // per row and stretch
     float *targets;                      // per row: the student's values at the teacher's k indices
 };
-
-template <typename E, bool NT>
-__device__ nbh_softmax stretch_stats(const typename E::item *in, int64_t begin, int64_t end, float scale)
-{
-    constexpr int kItems = E::items, kChunk = kThreads * kVecs * kItems;
-    nbh_softmax stats = nbh_softmax_empty();
-    for (int64_t at = begin; at < end; at += kChunk) {
-        float f[kVecs * kItems];
-        for (int j = 0; j < kVecs; ++j)
-            nbh_row_load<E, NT>(in, at + (j * kThreads + threadIdx.x) * kItems, end, -INFINITY,
-                                *reinterpret_cast<float(*)[kItems]>(f + j * kItems));
-        nbh_softmax_add(stats, f, scale);
-    }
-    return stats;
-}
 
 template <typename E>
 __global__ __launch_bounds__(kThreads) void distill_stats(Distill a)
@@ -58,7 +44,7 @@ __global__ __launch_bounds__(kThreads) void distill_stats(Distill a)
     const typename E::item *in = reinterpret_cast<const typename E::item *>(a.student + row * a.stride);
     const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
     const nbh_softmax stats =
-        nbh_softmax_group<kThreads>(stretch_stats<E, false>(in, begin, end, a.scale), a.scale, room);
+        nbh_softmax_group<kThreads>(nbh_row_stats<E, kThreads, false>(in, begin, end, a.scale), a.scale, room);
     if (threadIdx.x == 0)
         a.parts[(row - a.row0) * a.splits + split] = stats;
     // The loss needs these of the whole row, and the gradient may be written over the row while another
@@ -118,7 +104,7 @@ template <typename E, int WHAT>
 __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
 {
     typedef typename E::item item;
-    constexpr int kItems = E::items, kChunk = kThreads * kVecs * kItems;
+    constexpr int kItems = E::items;
     extern __shared__ char lds[];        // index, p and log p, and the table that finds repeated indices
     __shared__ nbh_softmax room[kWaves];
     __shared__ float add_room[kWaves];
@@ -176,8 +162,8 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
     }
     some = __syncthreads_or(some);
 
-    // -- the student's statistics: exp(s / T - lse) = base * 2^((s - shift) * scale)
-    float shift, base, log_sum = 0.0f;
+    // -- the student's statistics: exp(s / T - lse) = base * 2^(s * scale - peak * scale)
+    float peak_s, base, log_sum = 0.0f;
     if (WHAT & kLoss) {
         nbh_softmax stats;
         if (WHAT & kParts) {
@@ -185,22 +171,32 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
             for (int s = 1; s < a.splits; ++s)
                 stats = nbh_softmax_join(stats, a.parts[(row - a.row0) * a.splits + s], a.scale);
         } else {
-            stats = nbh_softmax_group<kThreads>(stretch_stats<E, false>(in, 0, a.vocab, a.scale), a.scale, room);
+            stats = nbh_softmax_group<kThreads>(nbh_row_stats<E, kThreads, false>(in, 0, a.vocab, a.scale), a.scale,
+                                                room);
         }
-        shift = stats.peak;
+        peak_s = stats.peak == -INFINITY ? 0.0f : stats.peak;
         base = stats.sum == 0.0f ? 0.0f : 1.0f / stats.sum;
-        log_sum = logf(stats.sum);
+        log_sum = log2f(stats.sum);
         if (a.lse && split == 0 && threadIdx.x == 0)
-            a.lse[row] = stats.peak / a.temperature + log_sum;
+            a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     } else {
         const float lse = a.lse[row];
-        // T * lse rounded to float32, and what the rounding took off put into the factor
-        shift = lse * a.temperature;
-        const float rest = __builtin_isfinite(shift) ? fmaf(lse, a.temperature, -shift) : 0.0f;
-        base = expf(-rest / a.temperature);
+        // T * lse rounded to float32 takes the place of the largest value; what the roundings of it, of
+        // its product with the scale, and of the scale itself take off goes into the factor.
+        peak_s = lse * a.temperature;
+        const float product = peak_s * a.scale;
+        if (nbh_softmax_near(product)) {
+            const float high = lse * kLog2e, low = fmaf(lse, kLog2e, -high) + lse * kLog2eRest;
+            base = exp2f((product - high) - low + peak_s * a.scale_rest);
+        } else {
+            const float rest = __builtin_isfinite(peak_s) ? fmaf(lse, a.temperature, -peak_s) : 0.0f;
+            base = expf(-rest / a.temperature);
+        }
         if (lse == -INFINITY)
-            shift = base = 0.0f;
+            peak_s = base = 0.0f;
     }
+    const float product = peak_s * a.scale;
+    const bool near = nbh_softmax_near(product);
 
     // -- loss
     if ((WHAT & kLoss) && split == 0) {
@@ -208,7 +204,11 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
         for (int j = threadIdx.x; j < a.k; j += kThreads)
             if (index[j] >= 0 && p[j] != 0.0f) {
                 const float s = WHAT & kParts ? a.targets[(row - a.row0) * a.k + j] : E::get(in[index[j]]);
-                const float log_q = s == -INFINITY ? s : (s - shift) / a.temperature - log_sum;
+                float log_q = s;
+                if (s != -INFINITY)
+                    log_q = near && fabsf(s) < 1e30f
+                                ? (fmaf(s, a.scale, -product) - log_sum) * kLn2
+                                : (s - peak_s) / a.temperature - log_sum * kLn2;
                 loss += p[j] * (log_p[j] - log_q);
             }
         loss = group_add(loss, add_room);
@@ -270,19 +270,25 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
             }
         }
         const float s = E::get(in[index[j]]);
-        log_p[j] = whole * nbh_exp2((s - shift) * a.scale) - factor * own;
+        log_p[j] = whole * nbh_softmax_term(s, peak_s, a.scale) - factor * own;
     }
     __syncthreads();
-    for (int64_t at = begin; at < end; at += kChunk) {
-        float f[kVecs][kItems];
-        for (int j = 0; j < kVecs; ++j)
-            nbh_row_load<E, false>(in, at + (j * kThreads + threadIdx.x) * kItems, end, 0.0f, f[j]);
-        for (int j = 0; j < kVecs; ++j) {
-            for (int i = 0; i < kItems; ++i)
-                f[j][i] = whole * nbh_exp2((f[j][i] - shift) * a.scale);
-            nbh_row_store<E, true>(out, at + (j * kThreads + threadIdx.x) * kItems, end, f[j]);
+    nbh_row_stream<E, kThreads, false>(in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) {
+#pragma unroll
+        for (int j = 0; j < kNbhAhead; ++j) {
+            float f[kItems];
+            E::unpack(raw[j], f);
+            if (near) {
+#pragma unroll
+                for (int i = 0; i < kItems; ++i)
+                    f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+            } else {
+                for (int i = 0; i < kItems; ++i)
+                    f[i] = whole * nbh_exp2((f[i] - peak_s) * a.scale);
+            }
+            nbh_row_store<E, true>(out, at + (j * kThreads + threadIdx.x) * kItems, end, f);
         }
-    }
+    });
     __syncthreads();
     for (int j = threadIdx.x; j < a.k; j += kThreads) {
         if (index[j] < begin || index[j] >= end)
@@ -305,7 +311,7 @@ struct Split {
 };
 Split split_of(int64_t rows, int64_t vocab, int dtype)
 {
-    const int64_t chunk = (int64_t)kThreads * kVecs * (dtype == NBH_ROW_F32 ? 4 : 8);
+    const int64_t chunk = (int64_t)kThreads * kNbhAhead * (dtype == NBH_ROW_F32 ? 4 : 8);
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
@@ -392,7 +398,8 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     a.grad_loss_stride = p->grad_loss_stride;
     a.grad_loss_value = (float)p->grad_loss_value;
     a.temperature = (float)p->temperature;
-    a.scale = (float)(1.4426950408889634 / p->temperature);
+    a.scale = (float)(1.4426950408889634 / a.temperature);
+    a.scale_rest = (float)(1.4426950408889634 / a.temperature - a.scale);
     a.loss = p->loss;
     a.lse = p->lse;
     a.grad = (char *)p->grad;

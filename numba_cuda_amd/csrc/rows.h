@@ -157,39 +157,75 @@ __device__ __forceinline__ void nbh_row_store(typename E::item *row, int64_t at,
     }
 }
 
-// Running softmax statistics: `peak` is the largest value so far, kept finite so that no difference of
-// infinities arises, `sum` is sum 2^((x - peak) * scale) with scale = log2(e) / temperature.  Subtracting
-// before scaling keeps the exponent exact at the peak, also for rows filled with the type's lowest value.
-// A NaN stays in `sum`; a row of -inf has sum 0; +inf makes it inf.
+// Running softmax statistics of values x, with scale = log2(e) / temperature: `sum` is the sum of
+// 2^(x scale - peak scale) for a reference `peak` (-inf before the first value above -inf), which is at
+// most 64 powers of two below the largest value: it is raised only when a value would exceed that, so that
+// nearly all values cost one fused multiply-add, one exponential and one addition.  The product peak scale
+// is rounded once and used so everywhere, which makes the rounding harmless.  Where it would overflow
+// (rows filled with the type's lowest value) differences x - peak are formed first instead.
+// A NaN stays in `sum`; a row of -inf has peak -inf and sum 0; +inf makes `sum` inf.
 struct nbh_softmax {
     float peak, sum;
 };
-__device__ __forceinline__ nbh_softmax nbh_softmax_empty() { return {-FLT_MAX, 0.0f}; }
+__device__ __forceinline__ nbh_softmax nbh_softmax_empty() { return {-INFINITY, 0.0f}; }
 __device__ __forceinline__ float nbh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-template <int N>
-__device__ __forceinline__ void nbh_softmax_add(nbh_softmax &s, const float (&f)[N], float scale)
+__device__ __forceinline__ bool nbh_softmax_near(float product) { return fabsf(product) < 1e30f; }
+// 2^(x scale - peak scale)
+__device__ __forceinline__ float nbh_softmax_term(float x, float peak, float scale)
 {
-    float peak = f[0];
-    for (int i = 1; i < N; ++i)
-        peak = fmaxf(peak, f[i]);
-    peak = fmaxf(s.peak, fminf(peak, FLT_MAX));
-    float sum[2] = {0.0f, 0.0f};
-    for (int i = 0; i < N; i += 2) {
-        sum[0] += nbh_exp2((f[i] - peak) * scale);
-        sum[1] += nbh_exp2((f[i + 1] - peak) * scale);
+    const float product = peak * scale;
+    return nbh_exp2(nbh_softmax_near(product) ? fmaf(x, scale, -product) : (x - peak) * scale);
+}
+__device__ __forceinline__ float nbh_softmax_factor(float from, float to, float scale)
+{
+    const float a = from * scale, b = to * scale;
+    return nbh_exp2(nbh_softmax_near(a) && nbh_softmax_near(b) ? a - b : (from - to) * scale);
+}
+// Values f, the largest of which is `most` (or NaN).
+template <int N>
+__device__ __forceinline__ void nbh_softmax_add(nbh_softmax &s, const float (&f)[N], float most, float scale)
+{
+    // 64 powers of two above the reference
+    if (__any(!(most <= fmaf(64.0f, __builtin_amdgcn_rcpf(scale), s.peak)))) {
+        const float peak = fmaxf(s.peak, fminf(most, FLT_MAX));
+        if (peak != s.peak) {
+            s.sum *= nbh_softmax_factor(s.peak, peak, scale);
+            s.peak = peak;
+        }
     }
-    s.sum = s.sum * nbh_exp2((s.peak - peak) * scale) + (sum[0] + sum[1]);
-    s.peak = peak;
+    const float product = s.peak == -INFINITY ? 0.0f : s.peak * scale;
+    float sum[2] = {0.0f, 0.0f};
+    if (__any(!nbh_softmax_near(product))) {
+        for (int i = 0; i < N; ++i)
+            sum[i & 1] += s.peak == -INFINITY ? nbh_exp2(f[i]) : nbh_softmax_term(f[i], s.peak, scale);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            sum[i & 1] += nbh_exp2(fmaf(f[i], scale, -product));
+    }
+    s.sum += sum[0] + sum[1];
+}
+template <int N> __device__ __forceinline__ float nbh_row_most(const float (&f)[N])
+{
+    float most = f[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i)
+        most = __builtin_elementwise_maximum(most, f[i]);
+    return most;
 }
 __device__ __forceinline__ nbh_softmax nbh_softmax_join(nbh_softmax a, nbh_softmax b, float scale)
 {
     const float peak = fmaxf(a.peak, b.peak);
-    return {peak, a.sum * nbh_exp2((a.peak - peak) * scale) + b.sum * nbh_exp2((b.peak - peak) * scale)};
+    if (peak == -INFINITY)
+        return {peak, a.sum + b.sum};
+    return {peak, a.sum * nbh_softmax_factor(a.peak, peak, scale) + b.sum * nbh_softmax_factor(b.peak, peak, scale)};
 }
 // log sum exp(x / temperature)
-__device__ __forceinline__ float nbh_softmax_lse(nbh_softmax s, float temperature)
+__device__ __forceinline__ float nbh_softmax_lse(nbh_softmax s, float temperature, float scale)
 {
-    return s.peak / temperature + logf(s.sum);
+    const float product = s.peak * scale;
+    return nbh_softmax_near(product) ? (product + log2f(s.sum)) * 0.693147180559945309f
+                                     : s.peak / temperature + logf(s.sum);
 }
 // Over a workgroup of `T` lanes; `room` holds T / 64 entries.  Every lane gets the result.
 template <int T>
@@ -206,6 +242,53 @@ __device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float sc
     for (int w = 1; w < T / 64; ++w)
         s = nbh_softmax_join(s, room[w], scale);
     return s;
+}
+
+// A workgroup of T lanes goes through elements begin .. end of a row in chunks of `kNbhAhead` 16-byte
+// vectors per lane, the next chunk on its way while the last is looked at: chunk(at, raw), where vector j
+// of a lane starts at element at + (j T + lane) items.  What lies behind the end reads as -inf.
+constexpr int kNbhAhead = 4;
+template <typename E, int T, bool NT, typename F>
+__device__ __forceinline__ void nbh_row_stream(const typename E::item *in, int64_t begin, int64_t end, F chunk)
+{
+    constexpr int kChunk = kNbhAhead * T * E::items;
+    auto ask = [&](nbh_u32x4(&to)[kNbhAhead], int64_t at) {
+        if (at + kChunk <= end) {
+#pragma unroll
+            for (int j = 0; j < kNbhAhead; ++j)
+                to[j] = E::template load<NT>(in + at + (j * T + threadIdx.x) * E::items);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kNbhAhead; ++j)
+                to[j] = nbh_row_load_raw<E, NT>(in, at + (j * T + threadIdx.x) * E::items, end, E::lowest);
+        }
+    };
+    nbh_u32x4 raw[kNbhAhead], next[kNbhAhead];
+    if (begin < end)
+        ask(raw, begin);
+#pragma unroll 1
+    for (int64_t at = begin; at < end; at += kChunk) {
+        if (at + kChunk < end)
+            ask(next, at + kChunk);
+        chunk(at, raw);
+#pragma unroll
+        for (int j = 0; j < kNbhAhead; ++j)
+            raw[j] = next[j];
+    }
+}
+template <typename E, int T, bool NT>
+__device__ __forceinline__ nbh_softmax nbh_row_stats(const typename E::item *in, int64_t begin, int64_t end, float scale)
+{
+    nbh_softmax stats = nbh_softmax_empty();
+    nbh_row_stream<E, T, NT>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kNbhAhead]) {
+#pragma unroll
+        for (int j = 0; j < kNbhAhead; ++j) {
+            float f[E::items];
+            E::unpack(raw[j], f);
+            nbh_softmax_add(stats, f, nbh_row_most(f), scale);
+        }
+    });
+    return stats;
 }
 
 // Temperatures whose reciprocal is an ordinary float32 number.

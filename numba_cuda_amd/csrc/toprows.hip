@@ -1,50 +1,49 @@
 // nbh_rows_top: the k largest entries of each row of logits with their indices, and the row's log-sum-exp.
 //
 // Entries are compared as 64-bit integers, (an integer that orders like the value) << 32 | ~index: no two
-// are equal, so ties and NaN need no cases of their own.  A workgroup reads a stretch of a row once and
-// keeps the maximum of each 16-byte vector:
-//   * The maxima of the lanes (or of the parts of a lane, for large k) are maxima of disjoint groups, so the
-//     k-th largest of them is a value that at least k entries reach, and hardly more: with m groups about
-//     -m ln(1 - k / m).  Bisection on the integers finds it, or one a little below, in a few counts.
-//   * The vectors whose maximum reaches it are read again (about k of them), what reaches it in them is
+// are equal, so ties and NaN need no cases of their own.  The row is read once:
+//   * The entries are split into groups (what a lane reads in a number of chunks), whose maxima are kept.
+//     The k-th largest of the maxima is a value that at least k entries reach, and hardly more: with m
+//     groups about -m ln(1 - k / m).  Bisection on the integers finds it, or one a little below, in a few
+//     counts.
+//   * The groups whose maximum reaches it are read again (about k of them); what reaches it there is
 //     appended to a list in LDS, whose order does not matter, and the list is sorted: short ones by
 //     counting how many entries exceed each, others by a bitonic network.
 //   * Where too many entries reach it (masses of equal ones, rows sorted by blocks) the bound is raised by
 //     bisection over all entries, and if it ends on a value that too many share, over their indices.
-// Rows longer than a stretch, and few rows, are split over workgroups, whose lists a second launch joins.
+// Many rows: one workgroup does all of that for a row.  Few rows: a first launch spreads the groups'
+// maxima and the statistics of the log-sum-exp over the device, a second one does the rest.
 #include "rows.h"
 
 namespace {
 
-constexpr int kJoinThreads = 256;
-constexpr int kJoinCap = 4096;           // entries the joining workgroup holds at a time
+constexpr int kAhead = kNbhAhead;
+constexpr int kSlots = 16;               // groups per lane that the one-launch kernel remembers
+constexpr int kMaximaThreads = 256;      // first launch of two
+constexpr int kMostGroups = 16384;       // groups per row of the two-launch path
+constexpr int kFinishThreads = 1024;
 
 struct Top {
     const char *in;
-    int64_t stride, vocab, slice, row0;
-    int splits, k;
+    int64_t stride, vocab, row0;
+    int k;
     char *values;
     int64_t values_stride;
     char *indices;
     int64_t indices_stride;
     float *lse;
     float temperature, scale;
-    uint64_t *parts;                     // splits lists of k per row, when rows are split
-    nbh_softmax *part_stats;
+    int splits, parts;                   // two launches: workgroups per row, groups per lane of theirs
+    int64_t slice;                       // entries per workgroup
+    uint32_t *maxima;                    // [row][split][part][lane], as keys, 0 for an empty group
+    nbh_softmax *part_stats;             // [row][split]
 };
 
-// Orders like the value; NaN above all, -0 as +0.
+// Orders like the value; NaN above all, -0 as +0.  No value has key 0.
 __device__ __forceinline__ uint32_t key_of(float x)
 {
     const uint32_t bits = __float_as_uint(x + 0.0f);
     return x != x ? 0xffffffffu : bits ^ ((uint32_t)((int32_t)bits >> 31) | 0x80000000u);
-}
-// A float `t` such that !(x < t) holds for every x whose key reaches `key` (and, if t is NaN, for all).
-__device__ __forceinline__ float float_at(uint32_t key)
-{
-    if (key <= 0x007fffffu)              // -inf's key or below
-        return __uint_as_float(0xff800000u);
-    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 __device__ __forceinline__ uint64_t entry_of(float x, int64_t index)
 {
@@ -74,45 +73,135 @@ template <int T> __device__ __forceinline__ int group_sum(int of_wave, Shared<T>
     return sum;
 }
 
-// Cuts the list (`have` entries, more than k) to its k best, in any order.
-template <int T, int CAP> __device__ void cut_list(uint64_t *list, int have, int k, Shared<T> &sh, int &turn)
+// A key that at least k of the groups' maxima reach (P of them in every lane, 0 for none), or 1 if there
+// are not that many; `top` is the largest.
+template <int T, int P>
+__device__ uint32_t bound_of(const uint32_t (&peaks)[P], int k, Shared<T> &sh, int &turn, uint32_t &top)
 {
-    uint64_t mine[CAP / T];
-    for (int i = 0; i < CAP / T; ++i) {
-        const int at = i * T + threadIdx.x;
-        mine[i] = at < have ? list[at] : 0;
+    uint32_t high = 0, low = ~0u;
+#pragma unroll
+    for (int g = 0; g < P; ++g) {
+        high = peaks[g] > high ? peaks[g] : high;
+        low = peaks[g] && peaks[g] < low ? peaks[g] : low;
     }
-    uint64_t low = 1, high = ~0ull;      // at least k entries reach `low`, fewer `high` + 1
+    for (int step = 32; step; step >>= 1) {
+        const uint32_t h = __shfl_xor(high, step), l = __shfl_xor(low, step);
+        high = h > high ? h : high;
+        low = l < low ? l : low;
+    }
+    int there = 0;
+#pragma unroll
+    for (int g = 0; g < P; ++g)
+        there += __popcll(__ballot(peaks[g] != 0));
+    if ((threadIdx.x & 63) == 0) {
+        sh.ends[0][threadIdx.x >> 6] = high;
+        sh.ends[1][threadIdx.x >> 6] = low;
+    }
+    there = group_sum(there, sh, turn);
+    for (int w = 0; w < T / 64; ++w) {
+        high = sh.ends[0][w] > high ? sh.ends[0][w] : high;
+        low = sh.ends[1][w] < low ? sh.ends[1][w] : low;
+    }
+    top = high;
+    if (there < k)
+        return 1;
     while (low < high) {
-        const uint64_t mid = high - (high - low) / 2;
+        const uint32_t mid = high - (high - low) / 2;
         int reach = 0;
-        for (int i = 0; i < CAP / T; ++i)
-            reach += __popcll(__ballot(mine[i] >= mid));
+#pragma unroll
+        for (int g = 0; g < P; ++g)
+            reach += __popcll(__ballot(peaks[g] >= mid));
         reach = group_sum(reach, sh, turn);
         if (reach >= k)
             low = mid;
         else
             high = mid - 1;
-        if (reach == k)
+        if (reach >= k && reach <= k + k / 8)
             break;
     }
-    __syncthreads();                     // everybody has read the list
-    if (threadIdx.x == 0)
-        sh.count = 0;
-    __syncthreads();
-    for (int i = 0; i < CAP / T; ++i)
-        if (mine[i] >= low)
-            list[atomicAdd(&sh.count, 1)] = mine[i];
-    __syncthreads();
+    return low;
 }
 
-// Calls put(rank, entry) for the k best of the list, rank 0 the largest; fewer if there are fewer.  The
-// list has been written before a barrier and has room for two entries more.
-template <int T, int CAP, typename F>
-__device__ void rank_list(uint64_t *list, int have, int k, Shared<T> &sh, int &turn, F put)
+// Appends what reaches `bound` of the entries at .. at + items.
+template <typename E, int T, int CAP>
+__device__ __forceinline__ void append(const typename E::item *in, int64_t at, int64_t end, uint64_t bound,
+                                       uint64_t *list, Shared<T> &sh)
 {
-    if (have <= T) {
-        // every lane counts what exceeds its entry: have / 2 reads of LDS, the same address in all lanes
+    if (at >= end)
+        return;
+    float f[E::items];
+    nbh_row_load<E, false>(in, at, end, -INFINITY, f);
+    if (key_of(nbh_row_most(f)) < (uint32_t)(bound >> 32))
+        return;
+    for (int i = 0; i < E::items; ++i) {
+        const uint64_t entry = entry_of(f[i], at + i);
+        if (entry >= bound && at + i < end) {
+            const int place = atomicAdd(&sh.count, 1);
+            if (place < CAP)
+                list[place] = entry;
+        }
+    }
+}
+
+// More than CAP of the row's n entries reach the key `low`, none exceeds the key `high`: a bound that at
+// least k and at most CAP entries reach.
+template <typename E, int T, int CAP>
+__device__ uint64_t raised_bound(const typename E::item *in, int64_t n, uint32_t low, uint32_t high, int k,
+                                 Shared<T> &sh, int &turn)
+{
+    auto count = [&](auto reaches) {
+        int mine = 0;
+        for (int64_t at = (int64_t)threadIdx.x * E::items; at < n; at += T * E::items) {
+            float f[E::items];
+            nbh_row_load<E, false>(in, at, n, -INFINITY, f);
+            for (int i = 0; i < E::items; ++i)
+                mine += at + i < n && reaches(f[i], at + i);
+        }
+        for (int step = 32; step; step >>= 1)
+            mine += __shfl_xor(mine, step);
+        return group_sum(mine, sh, turn);
+    };
+    int reach = CAP + 1;
+    while (low < high && reach > CAP) {
+        const uint32_t mid = high - (high - low) / 2;
+        const int now = count([&](float x, int64_t) { return key_of(x) >= mid; });
+        if (now >= k) {
+            low = mid;
+            reach = now;
+        } else {
+            high = mid - 1;
+        }
+    }
+    uint64_t from = (uint64_t)low << 32, to = from | 0xffffffffu;
+    while (from < to && reach > CAP) {   // low is the k-th largest value, and too many share it
+        const uint64_t mid = to - (to - from) / 2;
+        const int now = count([&](float x, int64_t index) { return entry_of(x, index) >= mid; });
+        if (now >= k) {
+            from = mid;
+            reach = now;
+        } else {
+            to = mid - 1;
+        }
+    }
+    return from;
+}
+
+// Writes the k best of the list (at least k entries) in order.  The list has been written before a
+// barrier and has room for two entries more.
+template <typename E, int T>
+__device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have)
+{
+    typedef typename E::item item;
+    const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
+    item *values = reinterpret_cast<item *>(a.values + row * a.values_stride);
+    int32_t *indices = reinterpret_cast<int32_t *>(a.indices + row * a.indices_stride);
+    auto put = [&](int rank, uint64_t entry) {
+        const int64_t index = index_of(entry);
+        values[rank] = in[index];
+        indices[rank] = (int32_t)index;
+    };
+    if (have <= 256) {
+        // a lane per entry counts what exceeds it: have / 2 reads of LDS, the same address in all lanes
         if (threadIdx.x == 0)
             list[have] = 0;
         __syncthreads();
@@ -123,336 +212,281 @@ __device__ void rank_list(uint64_t *list, int have, int k, Shared<T> &sh, int &t
                 const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list + i);
                 rank += (two.x > mine) + (two.y > mine);
             }
-            if (rank < k)
+            if (rank < a.k)
                 put(rank, mine);
         }
         return;
     }
-    int size = 2;
-    while (size < k)
-        size *= 2;
-    if (have > 2 * size) {
-        cut_list<T, CAP>(list, have, k, sh, turn);
-        have = sh.count;
-    }
+    int size = 512;
     while (size < have)
         size *= 2;
     for (int i = have + threadIdx.x; i < size; i += T)
         list[i] = 0;
+    __syncthreads();
     for (int run = 2; run <= size; run *= 2)
         for (int step = run / 2; step; step /= 2) {
-            __syncthreads();
             for (int i = threadIdx.x; i < size / 2; i += T) {
-                const int a = 2 * i - (i & (step - 1)), b = a + step;
-                const uint64_t x = list[a], y = list[b];
-                if ((x < y) == ((a & run) == 0)) {
-                    list[a] = y;
-                    list[b] = x;
+                const int at = 2 * i - (i & (step - 1)), other = at + step;
+                const uint64_t x = list[at], y = list[other];
+                if ((x < y) == ((at & run) == 0)) {
+                    list[at] = y;
+                    list[other] = x;
                 }
             }
+            // Pairs at most 64 apart stay within the 128 entries of a wavefront, whose LDS accesses are in
+            // order, until the next step reaches further.
+            if (step > 64 || (step == 1 && run >= 128))
+                __syncthreads();
+            else
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         }
     __syncthreads();
-    for (int i = threadIdx.x; i < k && i < have; i += T)
+    for (int i = threadIdx.x; i < a.k; i += T)
         put(i, list[i]);
 }
 
-template <typename E> struct Out {
-    typedef typename E::item item;
-    const item *in;
-    item *values;
-    int32_t *indices;
-    __device__ Out(const Top &a, int64_t row)
-        : in(reinterpret_cast<const item *>(a.in + row * a.stride)),
-          values(reinterpret_cast<item *>(a.values + row * a.values_stride)),
-          indices(reinterpret_cast<int32_t *>(a.indices + row * a.indices_stride))
-    {
-    }
-    __device__ void operator()(int rank, uint64_t entry) const
-    {
-        const int64_t index = index_of(entry);
-        values[rank] = in[index];
-        indices[rank] = (int32_t)index;
-    }
-};
-
-// T lanes take V vectors each; the maxima of P parts of a lane's vectors are its groups' maxima.
-template <typename E, bool LSE, int T, int V, int P, int CAP>
-__global__ __launch_bounds__(T, 4) void top_rows(Top a)
+// One workgroup per row.
+template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) void top_rows(Top a)
 {
     typedef typename E::item item;
-    constexpr int kItems = E::items, kAhead = 4;
+    constexpr int kItems = E::items, kChunk = kAhead * T * kItems;
     __shared__ __align__(16) uint64_t list[CAP + 2];
-    __shared__ float maxima[V * T];
+    __shared__ uint32_t maxima[kSlots * T];
     __shared__ Shared<T> sh;
-    const int64_t row = a.row0 + blockIdx.x / a.splits;
-    const int split = blockIdx.x % a.splits;
-    const int64_t begin = split * a.slice;
-    const item *in = reinterpret_cast<const item *>(a.in + row * a.stride) + begin;
-    const int n = (int)(a.vocab - begin < a.slice ? a.vocab - begin : a.slice);
+    const int64_t row = a.row0 + blockIdx.x;
+    const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
+    const int64_t n = a.vocab;
+    // chunks per group, a power of two
+    int shift = 0;
+    while ((n + kChunk - 1) / kChunk > (int64_t)kSlots << shift)
+        ++shift;
     int turn = 0;
-
     if (threadIdx.x == 0)
         sh.count = 0;
-    // -- the vectors' maxima, and the statistics of the log-sum-exp
-    nbh_softmax stats = nbh_softmax_empty();
-    float peak[P];
-#pragma unroll
-    for (int g = 0; g < P; ++g)
-        peak[g] = -INFINITY;
-    {
-        // four loads are on their way while four others are looked at
-        nbh_u32x4 raw[kAhead], next[kAhead];
-        auto ask = [&](nbh_u32x4(&to)[kAhead], int at) {
-            if ((at + kAhead * T) * kItems <= n) {
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    to[j] = E::template load<false>(in + (at + j * T + threadIdx.x) * kItems);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    to[j] = nbh_row_load_raw<E, false>(in, (at + j * T + threadIdx.x) * kItems, n, E::lowest);
-            }
-        };
-        ask(raw, 0);
-#pragma unroll 1
-        for (int at = 0; at * kItems < n; at += kAhead * T) {
-            if (V > kAhead)
-                ask(next, at + kAhead * T);
-            float part = -INFINITY;      // of this lane's four vectors
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j) {
-                float f[kItems];
-                E::unpack(raw[j], f);
-                float most = f[0];
-#pragma unroll
-                for (int i = 1; i < kItems; ++i)
-                    most = __builtin_elementwise_maximum(most, f[i]);
-                maxima[at + j * T + threadIdx.x] = most;
-                if (V == kAhead && P > 1)
-                    peak[j % P] = __builtin_elementwise_maximum(peak[j % P], most);
-                part = __builtin_elementwise_maximum(part, most);
-                if (LSE)
-                    nbh_softmax_add(stats, f, a.scale);
-            }
-            if (V > kAhead || P == 1) {
-#pragma unroll
-                for (int g = 0; g < P; ++g)
-                    if (at / (kAhead * T) % P == g)
-                        peak[g] = __builtin_elementwise_maximum(peak[g], part);
-            }
-#pragma unroll
-            for (int j = 0; j < kAhead; ++j)
-                raw[j] = next[j];
-        }
-    }
-    uint32_t peaks[P];
-    uint32_t high = 0, low = ~0u;
-#pragma unroll
-    for (int g = 0; g < P; ++g) {
-        // the group's first vector
-        const bool there = ((V > kAhead ? g * kAhead : g) * T + (int)threadIdx.x) * kItems < n;
-        peaks[g] = there ? key_of(peak[g]) : 0u;
-        high = peaks[g] > high ? peaks[g] : high;
-        low = peaks[g] < low ? peaks[g] : low;
-    }
-    // -- the bound: at least k of the maxima reach `low`, or it is below them all
-    for (int step = 32; step; step >>= 1) {
-        const uint32_t h = __shfl_xor(high, step), l = __shfl_xor(low, step);
-        high = h > high ? h : high;
-        low = l < low ? l : low;
-    }
-    if ((threadIdx.x & 63) == 0) {
-        sh.ends[0][threadIdx.x >> 6] = high;
-        sh.ends[1][threadIdx.x >> 6] = low;
-    }
-    __syncthreads();
-    for (int w = 0; w < T / 64; ++w) {
-        high = sh.ends[0][w] > high ? sh.ends[0][w] : high;
-        low = sh.ends[1][w] < low ? sh.ends[1][w] : low;
-    }
-    const uint32_t top = high;
-    if (low == 0 || a.k > T * P)
-        low = 1;                         // groups without entries, or fewer groups than entries wanted
-    if (a.k <= T * P)
-        while (low < high) {
-            const uint32_t mid = high - (high - low) / 2;
-            int reach = 0;
-#pragma unroll
-            for (int g = 0; g < P; ++g)
-                reach += __popcll(__ballot(peaks[g] >= mid));
-            reach = group_sum(reach, sh, turn);
-            if (reach >= a.k)
-                low = mid;
-            else
-                high = mid - 1;
-            if (reach >= a.k && reach <= a.k + a.k / 8)
-                break;
-        }
 
-    // -- what reaches it
-    uint64_t bound = (uint64_t)low << 32;
-    for (int attempt = 0;; ++attempt) {
-        const uint32_t key = (uint32_t)(bound >> 32);
-        const float from = float_at(key);
-        float lane = peak[0];
+    // -- groups' maxima, and the statistics of the log-sum-exp.  For the bound a lane's maximum will do up
+    // to k = T / 4, else the maxima of the four vectors of its chunks.
+    const bool fine = a.k > T / 4;
+    nbh_softmax stats = nbh_softmax_empty();
+    float peak[kAhead], slot = -INFINITY;
 #pragma unroll
-        for (int g = 1; g < P; ++g)
-            lane = __builtin_elementwise_maximum(lane, peak[g]);
-        // a lane sees its own maxima only
-        for (int v = threadIdx.x; !(lane < from) && v * kItems < n; v += T) {
-            if (maxima[v] < from)
-                continue;
-            const int first = v * kItems;
+    for (int j = 0; j < kAhead; ++j)
+        peak[j] = -INFINITY;
+    nbh_row_stream<E, T, false>(in, 0, n, [&](int64_t at, const nbh_u32x4(&raw)[kAhead]) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
             float f[kItems];
-            nbh_row_load<E, false>(in, first, n, -INFINITY, f);
-            for (int i = 0; i < kItems; ++i) {
-                const uint64_t entry = entry_of(f[i], begin + first + i);
-                if (entry >= bound && first + i < n) {
-                    const int place = atomicAdd(&sh.count, 1);
-                    if (place < CAP)
-                        list[place] = entry;
-                }
-            }
+            E::unpack(raw[j], f);
+            const float most = nbh_row_most(f);
+            peak[j] = __builtin_elementwise_maximum(peak[j], most);
+            slot = __builtin_elementwise_maximum(slot, most);
+            if (LSE)
+                nbh_softmax_add(stats, f, most, a.scale);
+        }
+        const int64_t chunk = at / kChunk;
+        maxima[(chunk >> shift) * T + threadIdx.x] = key_of(slot);
+        if (((chunk + 1) & ((1 << shift) - 1)) == 0)
+            slot = -INFINITY;
+    });
+    uint32_t peaks[kAhead], top;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        peaks[j] = (j * T + (int64_t)threadIdx.x) * kItems < n ? key_of(peak[j]) : 0u;
+    uint32_t key;
+    if (fine) {
+        key = bound_of<T>(peaks, a.k, sh, turn, top);
+    } else {
+        uint32_t lane[1] = {0u};
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j)
+            lane[0] = peaks[j] > lane[0] ? peaks[j] : lane[0];
+        key = bound_of<T>(lane, a.k, sh, turn, top);
+    }
+
+    // -- what reaches it: a lane reads its own groups again
+    uint64_t bound = (uint64_t)key << 32;
+    for (;;) {
+        const int64_t group = (int64_t)kChunk << shift;
+        for (int64_t g = 0; g * group < n; ++g) {
+            if (maxima[g * T + threadIdx.x] < (uint32_t)(bound >> 32))
+                continue;
+            for (int64_t at = g * group; at < (g + 1) * group && at < n; at += kChunk)
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j)
+                    append<E, T, CAP>(in, at + (j * T + (int64_t)threadIdx.x) * kItems, n, bound, list, sh);
         }
         __syncthreads();
-        if (sh.count <= CAP)
+        const int have = sh.count;
+        if (have <= CAP)
             break;
-        // Too many.  Raise the bound: first the value, until at most CAP entries reach it or it is the
-        // k-th largest, then the index, likewise.  (Two attempts: the second one's list is never too long.)
-        auto count = [&](auto reaches) {
-            int mine = 0;
-            for (int at = threadIdx.x * kItems; at < n; at += T * kItems) {      // from memory: this is rare
-                float f[kItems];
-                nbh_row_load<E, false>(in, at, n, -INFINITY, f);
-                for (int i = 0; i < kItems; ++i)
-                    mine += at + i < n && reaches(f[i], begin + at + i);
-            }
-            for (int step = 32; step; step >>= 1)
-                mine += __shfl_xor(mine, step);
-            return group_sum(mine, sh, turn);
-        };
-        uint32_t low = key, high = top;  // at least k entries reach `low`
-        int reach = CAP + 1;
-        while (low < high && reach > CAP) {
-            const uint32_t mid = high - (high - low) / 2;
-            const int now = count([&](float x, int64_t) { return key_of(x) >= mid; });
-            if (now >= a.k) {
-                low = mid;
-                reach = now;
-            } else {
-                high = mid - 1;
-            }
-        }
-        bound = (uint64_t)low << 32;
-        if (reach > CAP) {               // low is the k-th largest value, and too many share it
-            uint64_t from = bound, to = bound | 0xffffffffu;
-            while (from < to && reach > CAP) {
-                const uint64_t mid = to - (to - from) / 2;
-                const int now = count([&](float x, int64_t index) { return entry_of(x, index) >= mid; });
-                if (now >= a.k) {
-                    from = mid;
-                    reach = now;
-                } else {
-                    to = mid - 1;
-                }
-            }
-            bound = from;
-        }
+        bound = raised_bound<E, T, CAP>(in, n, (uint32_t)(bound >> 32), top, a.k, sh, turn);
+        __syncthreads();
         if (threadIdx.x == 0)
             sh.count = 0;
         __syncthreads();
     }
-    const int have = sh.count;
-    if (LSE)
+    if (LSE) {
         stats = nbh_softmax_group<T>(stats, a.scale, sh.stats);
-    if (a.splits == 1) {
-        rank_list<T, CAP>(list, have, a.k, sh, turn, Out<E>(a, row));
-        if (LSE && threadIdx.x == 0)
-            a.lse[row] = nbh_softmax_lse(stats, a.temperature);
-        return;
+        if (threadIdx.x == 0)
+            a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
-    uint64_t *part = a.parts + ((row - a.row0) * a.splits + split) * a.k;
-    rank_list<T, CAP>(list, have, a.k, sh, turn, [&](int rank, uint64_t entry) { part[rank] = entry; });
-    for (int i = have + threadIdx.x; i < a.k; i += T)
-        part[i] = 0;
-    if (LSE && threadIdx.x == 0)
-        a.part_stats[(row - a.row0) * a.splits + split] = stats;
+    write_ranked<E, T>(a, row, list, sh.count);
 }
 
-template <typename E, bool LSE> __global__ __launch_bounds__(kJoinThreads) void top_join(Top a)
+// First launch of two: the maxima of the lanes (or of the four vectors of their chunks) of a stretch.
+template <typename E, bool LSE> __global__ __launch_bounds__(kMaximaThreads) void top_maxima(Top a)
 {
-    constexpr int T = kJoinThreads;
-    __shared__ __align__(16) uint64_t list[kJoinCap + 2];
+    constexpr int T = kMaximaThreads, kItems = E::items;
+    __shared__ nbh_softmax room[T / 64];
+    const int64_t at = blockIdx.x / a.splits, row = a.row0 + at;
+    const int split = blockIdx.x % a.splits;
+    const typename E::item *in = reinterpret_cast<const typename E::item *>(a.in + row * a.stride);
+    const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
+    nbh_softmax stats = nbh_softmax_empty();
+    float peak[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+        peak[j] = -INFINITY;
+    nbh_row_stream<E, T, false>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kAhead]) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+            float f[kItems];
+            E::unpack(raw[j], f);
+            const float most = nbh_row_most(f);
+            peak[j] = __builtin_elementwise_maximum(peak[j], most);
+            if (LSE)
+                nbh_softmax_add(stats, f, most, a.scale);
+        }
+    });
+    uint32_t *out = a.maxima + (blockIdx.x * (int64_t)a.parts) * T + threadIdx.x;
+    uint32_t lane = 0;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+        const uint32_t key = begin + (j * T + (int64_t)threadIdx.x) * kItems < end ? key_of(peak[j]) : 0u;
+        lane = key > lane ? key : lane;
+        if (a.parts > 1)
+            out[j * T] = key;
+    }
+    if (a.parts == 1)
+        out[0] = lane;
+    if (LSE) {
+        stats = nbh_softmax_group<T>(stats, a.scale, room);
+        if (threadIdx.x == 0)
+            a.part_stats[at * a.splits + split] = stats;
+    }
+}
+
+// Second launch: a workgroup per row, P groups per lane.
+template <typename E, bool LSE, int P> __global__ __launch_bounds__(kFinishThreads) void top_finish(Top a)
+{
+    typedef typename E::item item;
+    constexpr int T = kFinishThreads, kItems = E::items, M = kMaximaThreads, CAP = 4096;
+    constexpr int kChunk = kAhead * M * kItems;
+    __shared__ __align__(16) uint64_t list[CAP + 2];
     __shared__ Shared<T> sh;
-    const int64_t at = blockIdx.x, row = a.row0 + at;
-    const int64_t all = (int64_t)a.splits * a.k;
+    const int64_t row = a.row0 + blockIdx.x;
+    const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
+    const int groups = a.splits * a.parts * M;
+    const uint32_t *maxima = a.maxima + blockIdx.x * (int64_t)groups;
+    int turn = 0;
+    if (threadIdx.x == 0)
+        sh.count = 0;
+    uint32_t peaks[P], top;
+#pragma unroll
+    for (int g = 0; g < P; ++g) {
+        const int at = g * T + threadIdx.x;
+        peaks[g] = at < groups ? maxima[at] : 0u;
+    }
+    uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
+    for (;;) {
+#pragma unroll 1
+        for (int g = threadIdx.x; g < groups; g += T) {
+            const uint32_t most = maxima[g];
+            if (most == 0 || most < (uint32_t)(bound >> 32))
+                continue;
+            const int lane = g % M, part = g / M % a.parts, split = g / M / a.parts;
+            const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
+            for (int64_t at = begin; at < end; at += kChunk)
+                if (a.parts > 1)
+                    append<E, T, CAP>(in, at + (part * M + lane) * kItems, end, bound, list, sh);
+                else
+#pragma unroll
+                    for (int j = 0; j < kAhead; ++j)
+                        append<E, T, CAP>(in, at + (j * M + lane) * kItems, end, bound, list, sh);
+        }
+        __syncthreads();
+        const int have = sh.count;
+        if (have <= CAP)
+            break;
+        bound = raised_bound<E, T, CAP>(in, a.vocab, (uint32_t)(bound >> 32), top, a.k, sh, turn);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            sh.count = 0;
+        __syncthreads();
+    }
     if (LSE && threadIdx.x == 0) {
         nbh_softmax stats = nbh_softmax_empty();
         for (int s = 0; s < a.splits; ++s)
-            stats = nbh_softmax_join(stats, a.part_stats[at * a.splits + s], a.scale);
-        a.lse[row] = nbh_softmax_lse(stats, a.temperature);
+            stats = nbh_softmax_join(stats, a.part_stats[blockIdx.x * (int64_t)a.splits + s], a.scale);
+        a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
-    int turn = 0, have = 0;
-    for (int64_t next = 0; next < all;) {
-        const int more = (int)(all - next < kJoinCap - have ? all - next : kJoinCap - have);
-        for (int i = threadIdx.x; i < more; i += T)
-            list[have + i] = a.parts[at * all + next + i];
-        __syncthreads();
-        next += more;
-        have += more;
-        if (next < all) {                // the list is full: keep its k best, all but the last list are whole
-            cut_list<T, kJoinCap>(list, have, a.k, sh, turn);
-            have = a.k;
-        }
-    }
-    rank_list<T, kJoinCap>(list, have, a.k, sh, turn, Out<E>(a, row));
+    write_ranked<E, T>(a, row, list, sh.count);
 }
 
-// Stretches a row is split into: 128 KiB on 512 lanes where rows alone make a workgroup or more per compute
-// unit, else 16 KiB on 256 lanes, unless
-// their lists would not fit the joining workgroup at once.
+// Workgroups per row: one from 256 rows on (a compute unit each), or where a row is a chunk or less; else
+// enough for four per compute unit, with at most kMostGroups groups.  Four groups per lane where k is more
+// than a quarter of the groups would otherwise be.
 struct Split {
-    bool large;
-    int splits;
+    int splits, parts;
     int64_t slice;
 };
 Split split_of(int64_t rows, int64_t vocab, int64_t k, int dtype)
 {
-    const int64_t items = dtype == NBH_ROW_F32 ? 4 : 8;
-    const int64_t small = 256 * 4 * items, large = 512 * 16 * items;
-    const int64_t many = (vocab + small - 1) / small, few = (vocab + large - 1) / large;
-    const bool use_large = many > 1 && (rows * few >= 256 || many * k > kJoinCap);
-    const int64_t splits = use_large ? few : many;
-    return {use_large, (int)splits, use_large ? large : small};
+    const int64_t chunk = (int64_t)kMaximaThreads * kAhead * (dtype == NBH_ROW_F32 ? 4 : 8);
+    const int64_t chunks = (vocab + chunk - 1) / chunk;
+    if (rows >= 256 || chunks == 1)
+        return {1, 1, vocab};
+    int64_t splits = (1024 + rows - 1) / rows;
+    if (splits > chunks)
+        splits = chunks;
+    if (splits > kMostGroups / kMaximaThreads)
+        splits = kMostGroups / kMaximaThreads;
+    int parts = k > splits * kMaximaThreads / 4 ? kAhead : 1;
+    if (parts * splits > kMostGroups / kMaximaThreads)
+        parts = 1;
+    const int64_t each = (chunks + splits - 1) / splits;
+    return {(int)((chunks + each - 1) / each), parts, each * chunk};
 }
 
-template <typename E, bool LSE>
-int launch_top(Top a, int64_t rows, bool large, hipStream_t stream)
+template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t stream)
 {
     const int64_t most = NBH_ROW_MOST_GROUPS / a.splits;
-    const int64_t all = rows;
-    for (a.row0 = 0; a.row0 < all; a.row0 += most) {
-        const int64_t now = all - a.row0 < most ? all - a.row0 : most;
-        const dim3 grid((unsigned)(now * a.splits));
-        if (large && a.k <= 256)
-            top_rows<E, LSE, 512, 16, 1, 2048><<<grid, dim3(512), 0, stream>>>(a);
-        else if (large)
-            top_rows<E, LSE, 512, 16, 4, 4096><<<grid, dim3(512), 0, stream>>>(a);
-        else if (a.k <= 128)
-            top_rows<E, LSE, 256, 4, 1, 2048><<<grid, dim3(256), 0, stream>>>(a);
-        else
-            top_rows<E, LSE, 256, 4, 4, 4096><<<grid, dim3(256), 0, stream>>>(a);
-        if (a.splits > 1)
-            top_join<E, LSE><<<dim3((unsigned)now), dim3(kJoinThreads), 0, stream>>>(a);
+    for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
+        const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
+        const dim3 grid((unsigned)now);
+        if (a.splits == 1) {
+            if (a.vocab <= 256 * kAhead * E::items && a.k <= 512)
+                top_rows<E, LSE, 256, 1024><<<grid, dim3(256), 0, stream>>>(a);
+            else if (a.k <= 512)
+                top_rows<E, LSE, 512, 1024><<<grid, dim3(512), 0, stream>>>(a);
+            else
+                top_rows<E, LSE, 512, 4096><<<grid, dim3(512), 0, stream>>>(a);
+        } else {
+            top_maxima<E, LSE><<<dim3((unsigned)(now * a.splits)), dim3(kMaximaThreads), 0, stream>>>(a);
+            const int groups = a.splits * a.parts * kMaximaThreads;
+            if (groups <= 4 * kFinishThreads)
+                top_finish<E, LSE, 4><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
+            else
+                top_finish<E, LSE, kMostGroups / kFinishThreads><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
+        }
         if (const int status = nbh_launch_status())
             return status;
     }
     return 0;
 }
-template <typename E>
-int launch_top(const Top &a, int64_t rows, bool large, hipStream_t stream)
+template <typename E> int launch_top(const Top &a, int64_t rows, hipStream_t stream)
 {
-    return a.lse ? launch_top<E, true>(a, rows, large, stream) : launch_top<E, false>(a, rows, large, stream);
+    return a.lse ? launch_top<E, true>(a, rows, stream) : launch_top<E, false>(a, rows, stream);
 }
 
 }  // namespace
@@ -463,7 +497,9 @@ extern "C" size_t nbh_rows_top_workspace(int64_t rows, int64_t vocab, int64_t k,
         dtype > NBH_ROW_BF16)
         return 0;
     const Split s = split_of(rows, vocab, k, dtype);
-    return s.splits == 1 ? 0 : (size_t)rows * s.splits * ((size_t)k * sizeof(uint64_t) + sizeof(nbh_softmax));
+    return s.splits == 1 ? 0
+                         : (size_t)rows * s.splits *
+                               ((size_t)s.parts * kMaximaThreads * sizeof(uint32_t) + sizeof(nbh_softmax));
 }
 
 extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int64_t stride, int dtype, int64_t k,
@@ -485,8 +521,6 @@ extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int
     a.in = (const char *)logits;
     a.stride = stride;
     a.vocab = vocab;
-    a.slice = split.slice;
-    a.splits = split.splits;
     a.k = (int)k;
     a.values = (char *)values;
     a.values_stride = values_stride;
@@ -494,18 +528,21 @@ extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int
     a.indices_stride = indices_stride;
     a.lse = lse;
     a.temperature = (float)temperature;
-    a.scale = (float)(1.4426950408889634 / temperature);
-    a.parts = (uint64_t *)workspace;
-    a.part_stats = (nbh_softmax *)((char *)workspace + (size_t)rows * split.splits * k * sizeof(uint64_t));
+    a.scale = (float)(1.4426950408889634 / a.temperature);
+    a.splits = split.splits;
+    a.parts = split.parts;
+    a.slice = split.slice;
+    a.maxima = (uint32_t *)workspace;
+    a.part_stats = (nbh_softmax *)(a.maxima + (size_t)rows * split.splits * split.parts * kMaximaThreads);
 
     const hipStream_t s = nbh_hip_stream(stream);
     nbh_stream_report report(s);
     switch (dtype) {
     case NBH_ROW_F32:
-        return launch_top<nbh_row_f32>(a, rows, split.large, s);
+        return launch_top<nbh_row_f32>(a, rows, s);
     case NBH_ROW_F16:
-        return launch_top<nbh_row_f16>(a, rows, split.large, s);
+        return launch_top<nbh_row_f16>(a, rows, s);
     default:
-        return launch_top<nbh_row_bf16>(a, rows, split.large, s);
+        return launch_top<nbh_row_bf16>(a, rows, s);
     }
 }
