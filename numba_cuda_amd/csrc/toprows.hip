@@ -6,9 +6,9 @@
 //     The k-th largest of the maxima is a value that at least k entries reach, and hardly more: with m
 //     groups about -m ln(1 - k / m).  Bisection on the integers finds it, or one a little below, in a few
 //     counts.
-//   * The groups whose maximum reaches it are read again (about k of them); what reaches it there is
-//     appended to a list in LDS, whose order does not matter, and the list is sorted: short ones by
-//     counting how many entries exceed each, others by a bitonic network.
+//   * The groups whose maximum reaches it, about k, are listed in LDS and read again, a vector per lane;
+//     what reaches it there is appended to another list, whose order does not matter, and that is sorted:
+//     short ones by counting how many entries exceed each, others by a bitonic network.
 //   * Where too many entries reach it (masses of equal ones, rows sorted by blocks) the bound is raised by
 //     bisection over all entries, and if it ends on a value that too many share, over their indices.
 // Many rows: one workgroup does all of that for a row.  Few rows: a first launch spreads the groups'
@@ -18,10 +18,10 @@
 namespace {
 
 constexpr int kAhead = kNbhAhead;
-constexpr int kSlots = 16;               // groups per lane that the one-launch kernel remembers
+constexpr int kSlots = 8;                // groups per lane that the one-launch kernel remembers
 constexpr int kMaximaThreads = 256;      // first launch of two
 constexpr int kMostGroups = 16384;       // groups per row of the two-launch path
-constexpr int kFinishThreads = 1024;
+constexpr int kFinishThreads = 512;
 
 struct Top {
     const char *in;
@@ -49,10 +49,17 @@ __device__ __forceinline__ uint64_t entry_of(float x, int64_t index)
 {
     return (uint64_t)key_of(x) << 32 | (uint32_t)~(uint32_t)index;
 }
+// The value again, but for the sign of a zero and the bits of a NaN.
+__device__ __forceinline__ float value_of(uint64_t entry)
+{
+    const uint32_t key = (uint32_t)(entry >> 32);
+    return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
 __device__ __forceinline__ int64_t index_of(uint64_t entry) { return (uint32_t)~(uint32_t)entry; }
 
 // What a workgroup of T lanes shares besides the list itself.
 template <int T> struct Shared {
+    int groups;                          // groups to be read again, or that would have been
     int count;                           // entries appended, or that would have been
     int tally[2][T / 64];                // by turn: counts of a bisection step
     uint32_t ends[2][T / 64];
@@ -116,7 +123,7 @@ __device__ uint32_t bound_of(const uint32_t (&peaks)[P], int k, Shared<T> &sh, i
             low = mid;
         else
             high = mid - 1;
-        if (reach >= k && reach <= k + k / 8)
+        if (reach >= k && reach <= k + (k < 64 ? 8 : k / 8))
             break;
     }
     return low;
@@ -197,7 +204,8 @@ __device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have
     int32_t *indices = reinterpret_cast<int32_t *>(a.indices + row * a.indices_stride);
     auto put = [&](int rank, uint64_t entry) {
         const int64_t index = index_of(entry);
-        values[rank] = in[index];
+        const float value = value_of(entry);
+        values[rank] = value == 0.0f || value != value ? in[index] : E::put(value);
         indices[rank] = (int32_t)index;
     };
     if (have <= 256) {
@@ -252,6 +260,7 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
     constexpr int kItems = E::items, kChunk = kAhead * T * kItems;
     __shared__ __align__(16) uint64_t list[CAP + 2];
     __shared__ uint32_t maxima[kSlots * T];
+    __shared__ int again[CAP];
     __shared__ Shared<T> sh;
     const int64_t row = a.row0 + blockIdx.x;
     const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
@@ -262,7 +271,7 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
         ++shift;
     int turn = 0;
     if (threadIdx.x == 0)
-        sh.count = 0;
+        sh.groups = sh.count = 0;
 
     // -- groups' maxima, and the statistics of the log-sum-exp.  For the bound a lane's maximum will do up
     // to k = T / 4, else the maxima of the four vectors of its chunks.
@@ -303,26 +312,31 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
         key = bound_of<T>(lane, a.k, sh, turn, top);
     }
 
-    // -- what reaches it: a lane reads its own groups again
+    // -- what reaches it
     uint64_t bound = (uint64_t)key << 32;
     for (;;) {
         const int64_t group = (int64_t)kChunk << shift;
-        for (int64_t g = 0; g * group < n; ++g) {
-            if (maxima[g * T + threadIdx.x] < (uint32_t)(bound >> 32))
-                continue;
-            for (int64_t at = g * group; at < (g + 1) * group && at < n; at += kChunk)
-#pragma unroll
-                for (int j = 0; j < kAhead; ++j)
-                    append<E, T, CAP>(in, at + (j * T + (int64_t)threadIdx.x) * kItems, n, bound, list, sh);
-        }
+        for (int g = threadIdx.x; (g / T) * group < n; g += T)
+            if (maxima[g] >= (uint32_t)(bound >> 32)) {
+                const int place = atomicAdd(&sh.groups, 1);
+                if (place < CAP)
+                    again[place] = g;
+            }
         __syncthreads();
-        const int have = sh.count;
-        if (have <= CAP)
-            break;
+        if (sh.groups <= CAP) {
+            const int vectors = kAhead << shift;     // of a group
+            for (int i = threadIdx.x; i < sh.groups * vectors; i += T) {
+                const int g = again[i / vectors], v = i % vectors;
+                append<E, T, CAP>(in, (g / T) * group + (v * T + g % T) * (int64_t)kItems, n, bound, list, sh);
+            }
+            __syncthreads();
+            if (sh.count <= CAP)
+                break;
+        }
         bound = raised_bound<E, T, CAP>(in, n, (uint32_t)(bound >> 32), top, a.k, sh, turn);
         __syncthreads();
         if (threadIdx.x == 0)
-            sh.count = 0;
+            sh.groups = sh.count = 0;
         __syncthreads();
     }
     if (LSE) {
@@ -383,6 +397,7 @@ template <typename E, bool LSE, int P> __global__ __launch_bounds__(kFinishThrea
     constexpr int T = kFinishThreads, kItems = E::items, M = kMaximaThreads, CAP = 4096;
     constexpr int kChunk = kAhead * M * kItems;
     __shared__ __align__(16) uint64_t list[CAP + 2];
+    __shared__ int again[CAP];
     __shared__ Shared<T> sh;
     const int64_t row = a.row0 + blockIdx.x;
     const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
@@ -390,45 +405,53 @@ template <typename E, bool LSE, int P> __global__ __launch_bounds__(kFinishThrea
     const uint32_t *maxima = a.maxima + blockIdx.x * (int64_t)groups;
     int turn = 0;
     if (threadIdx.x == 0)
-        sh.count = 0;
+        sh.groups = sh.count = 0;
     uint32_t peaks[P], top;
 #pragma unroll
     for (int g = 0; g < P; ++g) {
         const int at = g * T + threadIdx.x;
         peaks[g] = at < groups ? maxima[at] : 0u;
     }
-    uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
-    for (;;) {
-#pragma unroll 1
-        for (int g = threadIdx.x; g < groups; g += T) {
-            const uint32_t most = maxima[g];
-            if (most == 0 || most < (uint32_t)(bound >> 32))
-                continue;
-            const int lane = g % M, part = g / M % a.parts, split = g / M / a.parts;
-            const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
-            for (int64_t at = begin; at < end; at += kChunk)
-                if (a.parts > 1)
-                    append<E, T, CAP>(in, at + (part * M + lane) * kItems, end, bound, list, sh);
-                else
-#pragma unroll
-                    for (int j = 0; j < kAhead; ++j)
-                        append<E, T, CAP>(in, at + (j * M + lane) * kItems, end, bound, list, sh);
+    if (LSE && threadIdx.x < 64) {
+        static_assert(kMostGroups / M <= 64, "a lane per stretch");
+        const int lane = threadIdx.x;
+        nbh_softmax stats = lane < a.splits ? a.part_stats[blockIdx.x * (int64_t)a.splits + lane] : nbh_softmax_empty();
+        for (int step = 32; step; step >>= 1) {
+            const nbh_softmax other = {__shfl_xor(stats.peak, step), __shfl_xor(stats.sum, step)};
+            stats = nbh_softmax_join(stats, other, a.scale);
         }
+        if (lane == 0)
+            a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
+    }
+    uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
+    const int chunks = (int)(a.slice / kChunk), vectors = chunks * (a.parts > 1 ? 1 : kAhead);       // of a group
+    for (;;) {
+#pragma unroll
+        for (int g = 0; g < P; ++g)
+            if (peaks[g] && peaks[g] >= (uint32_t)(bound >> 32)) {
+                const int place = atomicAdd(&sh.groups, 1);
+                if (place < CAP)
+                    again[place] = g * T + threadIdx.x;
+            }
         __syncthreads();
-        const int have = sh.count;
-        if (have <= CAP)
-            break;
+        if (sh.groups <= CAP) {
+            for (int64_t i = threadIdx.x; i < (int64_t)sh.groups * vectors; i += T) {
+                const int g = again[i / vectors], v = (int)(i % vectors);
+                const int lane = g % M, part = g / M % a.parts, split = g / M / a.parts;
+                const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
+                const int64_t at = a.parts > 1 ? begin + v * (int64_t)kChunk + (part * M + lane) * kItems
+                                               : begin + (v * (int64_t)M + lane) * kItems;
+                append<E, T, CAP>(in, at, end, bound, list, sh);
+            }
+            __syncthreads();
+            if (sh.count <= CAP)
+                break;
+        }
         bound = raised_bound<E, T, CAP>(in, a.vocab, (uint32_t)(bound >> 32), top, a.k, sh, turn);
         __syncthreads();
         if (threadIdx.x == 0)
-            sh.count = 0;
+            sh.groups = sh.count = 0;
         __syncthreads();
-    }
-    if (LSE && threadIdx.x == 0) {
-        nbh_softmax stats = nbh_softmax_empty();
-        for (int s = 0; s < a.splits; ++s)
-            stats = nbh_softmax_join(stats, a.part_stats[blockIdx.x * (int64_t)a.splits + s], a.scale);
-        a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
     write_ranked<E, T>(a, row, list, sh.count);
 }
@@ -465,17 +488,17 @@ template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t 
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
         const dim3 grid((unsigned)now);
         if (a.splits == 1) {
-            if (a.vocab <= 256 * kAhead * E::items && a.k <= 512)
+            // 256 lanes make 1024 groups, which serve up to k = 256; larger workgroups wait longer at
+            // their barriers (4096 x 65536 bfloat16, k = 64: 124 us, with 512 lanes 140 us)
+            if (a.k <= 256)
                 top_rows<E, LSE, 256, 1024><<<grid, dim3(256), 0, stream>>>(a);
-            else if (a.k <= 512)
-                top_rows<E, LSE, 512, 1024><<<grid, dim3(512), 0, stream>>>(a);
             else
                 top_rows<E, LSE, 512, 4096><<<grid, dim3(512), 0, stream>>>(a);
         } else {
             top_maxima<E, LSE><<<dim3((unsigned)(now * a.splits)), dim3(kMaximaThreads), 0, stream>>>(a);
             const int groups = a.splits * a.parts * kMaximaThreads;
-            if (groups <= 4 * kFinishThreads)
-                top_finish<E, LSE, 4><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
+            if (groups <= 8 * kFinishThreads)
+                top_finish<E, LSE, 8><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
             else
                 top_finish<E, LSE, kMostGroups / kFinishThreads><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
         }
