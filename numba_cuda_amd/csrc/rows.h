@@ -247,40 +247,49 @@ __device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float sc
 // A workgroup of T lanes goes through elements begin .. end of a row in chunks of `kNbhAhead` 16-byte
 // vectors per lane, the next chunk on its way while the last is looked at: chunk(at, raw), where vector j
 // of a lane starts at element at + (j T + lane) items.  What lies behind the end reads as -inf.
+// Whole chunks take turns in two sets of registers, and no load in that loop is conditional: a copy from
+// one set to the other, or a load on one path only, would make the compiler wait for all of them.
 constexpr int kNbhAhead = 4;
 template <typename E, int T, bool NT, typename F>
 __device__ __forceinline__ void nbh_row_stream(const typename E::item *in, int64_t begin, int64_t end, F chunk)
 {
     constexpr int kChunk = kNbhAhead * T * E::items;
-    auto ask = [&](nbh_u32x4(&to)[kNbhAhead], int64_t at) {
-        if (at + kChunk <= end) {
-#pragma unroll
-            for (int j = 0; j < kNbhAhead; ++j)
-                to[j] = E::template load<NT>(in + at + (j * T + threadIdx.x) * E::items);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kNbhAhead; ++j)
-                to[j] = nbh_row_load_raw<E, NT>(in, at + (j * T + threadIdx.x) * E::items, end, E::lowest);
-        }
-    };
-    nbh_u32x4 raw[kNbhAhead], next[kNbhAhead];
-    if (begin < end)
-        ask(raw, begin);
-#pragma unroll 1
-    for (int64_t at = begin; at < end; at += kChunk) {
-        if (at + kChunk < end)
-            ask(next, at + kChunk);
-        chunk(at, raw);
+    auto ask = [&](nbh_u32x4(&to)[kNbhAhead], int64_t at) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kNbhAhead; ++j)
-            raw[j] = next[j];
+            to[j] = E::template load<NT>(in + at + (j * T + threadIdx.x) * E::items);
+    };
+    nbh_u32x4 a[kNbhAhead], b[kNbhAhead], tail[kNbhAhead];
+    int64_t left = (end - begin) / kChunk, at = begin;
+    if (left)
+        ask(a, at);
+#pragma unroll 1
+    for (; left > 2; left -= 2, at += 2 * kChunk) {
+        ask(b, at + kChunk);
+        chunk(at, a);
+        ask(a, at + 2 * kChunk);
+        chunk(at + kChunk, b);
     }
+    if (left == 2)
+        ask(b, at + kChunk);
+    const int64_t rest = at + left * kChunk;
+    if (rest < end)
+#pragma unroll
+        for (int j = 0; j < kNbhAhead; ++j)
+            tail[j] = nbh_row_load_raw<E, NT>(in, rest + (j * T + threadIdx.x) * E::items, end, E::lowest);
+    if (left)
+        chunk(at, a);
+    if (left == 2)
+        chunk(at + kChunk, b);
+    if (rest < end)
+        chunk(rest, tail);
 }
 template <typename E, int T, bool NT>
 __device__ __forceinline__ nbh_softmax nbh_row_stats(const typename E::item *in, int64_t begin, int64_t end, float scale)
 {
     nbh_softmax stats = nbh_softmax_empty();
-    nbh_row_stream<E, T, NT>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kNbhAhead]) {
+    nbh_row_stream<E, T, NT>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kNbhAhead])
+                                 __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kNbhAhead; ++j) {
             float f[E::items];

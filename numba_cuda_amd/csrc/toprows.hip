@@ -281,7 +281,7 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         peak[j] = -INFINITY;
-    nbh_row_stream<E, T, false>(in, 0, n, [&](int64_t at, const nbh_u32x4(&raw)[kAhead]) {
+    nbh_row_stream<E, T, false>(in, 0, n, [&](int64_t at, const nbh_u32x4(&raw)[kAhead]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             float f[kItems];
@@ -361,7 +361,7 @@ template <typename E, bool LSE> __global__ __launch_bounds__(kMaximaThreads) voi
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         peak[j] = -INFINITY;
-    nbh_row_stream<E, T, false>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kAhead]) {
+    nbh_row_stream<E, T, false>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kAhead]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             float f[kItems];
