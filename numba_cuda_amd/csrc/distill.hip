@@ -273,7 +273,7 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
         log_p[j] = whole * nbh_softmax_term(s, peak_s, a.scale) - factor * own;
     }
     __syncthreads();
-    nbh_row_stream<E, kThreads, false>(in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
+    nbh_row_stream<E, kThreads, false, true>(in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kNbhAhead; ++j) {
             float f[kItems];

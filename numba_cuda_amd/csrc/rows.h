@@ -249,39 +249,49 @@ __device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float sc
 // of a lane starts at element at + (j T + lane) items.  What lies behind the end reads as -inf.
 // Whole chunks take turns in two sets of registers, and no load in that loop is conditional: a copy from
 // one set to the other, or a load on one path only, would make the compiler wait for all of them.
+// BACK: from the end to the beginning, for a second reading of the row that finds the end of the first in
+// the caches.
 constexpr int kNbhAhead = 4;
-template <typename E, int T, bool NT, typename F>
+template <typename E, int T, bool NT, bool BACK = false, typename F>
 __device__ __forceinline__ void nbh_row_stream(const typename E::item *in, int64_t begin, int64_t end, F chunk)
 {
-    constexpr int kChunk = kNbhAhead * T * E::items;
+    constexpr int64_t kChunk = kNbhAhead * T * E::items, kStep = BACK ? -kChunk : kChunk;
     auto ask = [&](nbh_u32x4(&to)[kNbhAhead], int64_t at) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kNbhAhead; ++j)
             to[j] = E::template load<NT>(in + at + (j * T + threadIdx.x) * E::items);
     };
     nbh_u32x4 a[kNbhAhead], b[kNbhAhead], tail[kNbhAhead];
-    int64_t left = (end - begin) / kChunk, at = begin;
-    if (left)
-        ask(a, at);
-#pragma unroll 1
-    for (; left > 2; left -= 2, at += 2 * kChunk) {
-        ask(b, at + kChunk);
-        chunk(at, a);
-        ask(a, at + 2 * kChunk);
-        chunk(at + kChunk, b);
-    }
-    if (left == 2)
-        ask(b, at + kChunk);
-    const int64_t rest = at + left * kChunk;
-    if (rest < end)
+    int64_t left = (end - begin) / kChunk;
+    const int64_t rest = begin + left * kChunk;
+    auto ask_tail = [&]() __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kNbhAhead; ++j)
             tail[j] = nbh_row_load_raw<E, NT>(in, rest + (j * T + threadIdx.x) * E::items, end, E::lowest);
+    };
+    int64_t at = BACK ? rest - kChunk : begin;
+    if (BACK && rest < end)
+        ask_tail();
+    if (left)
+        ask(a, at);
+    if (BACK && rest < end)
+        chunk(rest, tail);
+#pragma unroll 1
+    for (; left > 2; left -= 2, at += 2 * kStep) {
+        ask(b, at + kStep);
+        chunk(at, a);
+        ask(a, at + 2 * kStep);
+        chunk(at + kStep, b);
+    }
+    if (left == 2)
+        ask(b, at + kStep);
+    if (!BACK && rest < end)
+        ask_tail();
     if (left)
         chunk(at, a);
     if (left == 2)
-        chunk(at + kChunk, b);
-    if (rest < end)
+        chunk(at + kStep, b);
+    if (!BACK && rest < end)
         chunk(rest, tail);
 }
 template <typename E, int T, bool NT>

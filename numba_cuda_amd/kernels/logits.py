@@ -45,16 +45,11 @@ _DISTILL = struct.Struct("@qqP4q2P5q2Pqdd3PqPq")      # struct nbh_rows_distill_
 
 # ---- arguments ---------------------------------------------------------------------------
 
-class _Array:
-    """Address, shape, byte strides and dtype of an argument, and what keeps it alive."""
+# A call of a few microseconds on the device should not take many on the host: arguments become plain
+# tuples (address, shape, byte strides, dtype, what keeps the memory alive), found by the class of the
+# argument; a torch tensor's attributes cost a tenth of what its interface dictionary does.
 
-    __slots__ = ("address", "shape", "strides", "dtype", "owner")
-
-    def __init__(self, address, shape, strides, dtype, owner):
-        self.address, self.shape, self.strides, self.dtype, self.owner = address, shape, strides, dtype, owner
-
-
-_foreign_dtypes = {}                         # dtype objects of other libraries -> np.dtype
+_foreign_dtypes = {}                         # dtype objects of other libraries -> (np.dtype, its item size)
 
 
 def _foreign_dtype(dtype):
@@ -63,129 +58,172 @@ def _foreign_dtype(dtype):
         found = bfloat16 if name == "bfloat16" else np.dtype(name)
     except TypeError:
         raise TypeError("unsupported dtype: %s" % (dtype,)) from None
-    _foreign_dtypes[dtype] = found
-    return found
+    _foreign_dtypes[dtype] = found, found.itemsize
+    return _foreign_dtypes[dtype]
+
+
+def _view_of_own(array):
+    try:
+        address = array.gpu_data.device_pointer
+    except AttributeError:
+        address = array.device_ctypes_pointer.value or 0
+    return address, array.shape, array.strides, array.dtype, array
+
+
+def _view_of_tensor(tensor):
+    if not tensor.is_cuda:
+        return None
+    dtype = tensor.dtype
+    dtype, size = _foreign_dtypes.get(dtype) or _foreign_dtype(dtype)
+    strides = tensor.stride()
+    if len(strides) == 1:
+        strides = (strides[0] * size,)
+    elif len(strides) == 2:
+        strides = (strides[0] * size, strides[1] * size)
+    else:
+        strides = tuple([n * size for n in strides])
+    return tensor.data_ptr(), tensor.shape, strides, dtype, tensor
+
+
+_views = {devicearray.DeviceNDArray: _view_of_own}       # class -> function
 
 
 def _device_view(obj):
-    """The _Array of something in device memory, None for anything else."""
+    """The tuple of something in device memory, None for anything else."""
+    view = _views.get(obj.__class__)
+    if view is not None:
+        return view(obj)
     if getattr(obj, "__cuda_ndarray__", False):
-        return _Array(obj.device_ctypes_pointer.value or 0, obj.shape, obj.strides, obj.dtype, obj)
-    if getattr(obj, "is_cuda", None) is True and hasattr(obj, "data_ptr"):
-        # a torch tensor: its attributes cost a tenth of what its interface dictionary does
-        dtype = _foreign_dtypes.get(obj.dtype) or _foreign_dtype(obj.dtype)
-        size = dtype.itemsize
-        return _Array(obj.data_ptr(), tuple(obj.shape), tuple([s * size for s in obj.stride()]), dtype, obj)
+        return _view_of_own(obj)
+    if hasattr(obj, "is_cuda") and hasattr(obj, "data_ptr") and hasattr(obj, "stride"):
+        _views[obj.__class__] = _view_of_tensor
+        return _view_of_tensor(obj)
     if hasattr(obj, "__cuda_array_interface__"):
-        array = devicearray.auto_device(obj)[0]
-        return _Array(array.device_ctypes_pointer.value or 0, array.shape, array.strides, array.dtype, array)
+        return _view_of_own(devicearray.auto_device(obj)[0])
     return None
 
 
 _several_devices = None
 
 
-def _checked_device(array, name):
+def _check_device(view, name):
     """Refuse memory of another device than the calling thread's."""
     global _several_devices
     if _several_devices is None:
         _several_devices = _driver.driver.get_device_count() > 1
-    if _several_devices and array.address:
+    if _several_devices and view[0]:
         where, here = ctypes.c_int(), ctypes.c_int()
         _driver.driver.nbh_get_device(ctypes.byref(here))
-        _driver.driver.nbh_pointer_device(array.address, ctypes.byref(where))
+        _driver.driver.nbh_pointer_device(view[0], ctypes.byref(where))
         if where.value != here.value:
             raise ValueError("%s is on device %d, the current device is %d" % (name, where.value, here.value))
-    return array
 
 
 def _input(obj, name, stream, dtype=None):
-    """The _Array of an input; what is on the host is copied over."""
-    array = _device_view(obj)
-    if array is None:
+    """The tuple of an input; what is on the host is copied over."""
+    view = _device_view(obj)
+    if view is None:
         host = np.asarray(obj) if dtype is None else np.asarray(obj, dtype=dtype)
         if not host.flags["C_CONTIGUOUS"]:
             host = np.ascontiguousarray(host)
-        array = _device_view(devicearray.auto_device(host, stream=stream)[0])
-    return _checked_device(array, name)
+        view = _device_view(devicearray.auto_device(host, stream=stream)[0])
+    if _several_devices is not False:
+        _check_device(view, name)
+    return view
 
 
 def _output(obj, name):
-    array = _device_view(obj)
-    if array is None:
+    view = _device_view(obj)
+    if view is None:
         raise TypeError("%s must be a device array" % name)
-    return _checked_device(array, name)
+    if _several_devices is not False:
+        _check_device(view, name)
+    return view
 
 
-def _as_rows(array, name, shape=None, dtypes=_ROW_DTYPE):
+def _as_rows(view, name, shape=None, dtypes=_ROW_DTYPE):
     """Check a 2-d operand; returns the bytes from row to row."""
-    if len(array.shape) != 2:
-        raise ValueError("%s must be a 2-d array, got %d-d" % (name, len(array.shape)))
-    if array.dtype not in dtypes:
-        raise TypeError("%s has unsupported dtype %s" % (name, array.dtype))
-    if shape is not None and array.shape != shape:
-        raise ValueError("%s has shape %s, expected %s" % (name, array.shape, shape))
-    size = array.dtype.itemsize
-    if array.shape[1] > 1 and array.strides[1] != size:
-        raise ValueError("the items of a row of %s must lie next to each other (strides %s)" % (name, array.strides))
-    if array.address % size or (array.shape[0] > 1 and array.strides[0] % size):
+    address, own_shape, strides, dtype, _ = view
+    if len(own_shape) != 2:
+        raise ValueError("%s must be a 2-d array, got %d-d" % (name, len(own_shape)))
+    if dtype not in dtypes:
+        raise TypeError("%s has unsupported dtype %s" % (name, dtype))
+    if shape is not None and own_shape != shape:
+        raise ValueError("%s has shape %s, expected %s" % (name, tuple(own_shape), tuple(shape)))
+    size = dtype.itemsize
+    rows, columns = own_shape
+    if columns > 1 and strides[1] != size:
+        raise ValueError("the items of a row of %s must lie next to each other (strides %s)" % (name, strides))
+    if address % size or (rows > 1 and strides[0] % size):
         raise ValueError("%s is not aligned to its item size" % name)
-    return array.strides[0] if array.shape[0] > 1 else 0
+    return strides[0] if rows > 1 else 0
 
 
-def _as_result_rows(array, name, shape, dtypes=_ROW_DTYPE):
-    stride = _as_rows(array, name, shape, dtypes)
-    if shape[0] > 1 and shape[1] and abs(stride) < shape[1] * array.dtype.itemsize:
-        raise ValueError("the rows of %s overlap (strides %s)" % (name, array.strides))
+def _as_result_rows(view, name, shape, dtypes=_ROW_DTYPE):
+    stride = _as_rows(view, name, shape, dtypes)
+    if shape[0] > 1 and shape[1] and abs(stride) < shape[1] * view[3].itemsize:
+        raise ValueError("the rows of %s overlap (strides %s)" % (name, view[2]))
     return stride
 
 
-def _as_vector(array, name, length, dtypes):
-    if len(array.shape) != 1:
-        raise ValueError("%s must be a 1-d array, got %d-d" % (name, len(array.shape)))
-    if array.dtype not in dtypes:
-        raise TypeError("%s has unsupported dtype %s" % (name, array.dtype))
-    if length is not None and array.shape[0] != length:
-        raise ValueError("%s has %d items, expected %d" % (name, array.shape[0], length))
-    if array.shape[0] > 1 and array.strides[0] != array.dtype.itemsize:
+def _as_vector(view, name, length, dtypes):
+    address, shape, strides, dtype, _ = view
+    if len(shape) != 1:
+        raise ValueError("%s must be a 1-d array, got %d-d" % (name, len(shape)))
+    if dtype not in dtypes:
+        raise TypeError("%s has unsupported dtype %s" % (name, dtype))
+    n = shape[0]
+    if length is not None and n != length:
+        raise ValueError("%s has %d items, expected %d" % (name, n, length))
+    size = dtype.itemsize
+    if n > 1 and strides[0] != size:
         raise ValueError("%s must have unit stride" % name)
-    if array.address % array.dtype.itemsize:
+    if address % size:
         raise ValueError("%s is not aligned to its item size" % name)
-    return array
+    return view
 
 
 _INTEGERS = (_int32, _int64)
 _FLOATS = (_float32,)
 
 
-def _extent(array):
-    low = high = array.address
-    for n, s in zip(array.shape, array.strides):
+def _extent(view):
+    """First and last + 1 address of the items."""
+    low, shape, strides, dtype, _ = view
+    high = low
+    for n, step in zip(shape, strides):
         if n == 0:
             return low, low
-        if s < 0:
-            low += (n - 1) * s
+        if step < 0:
+            low += (n - 1) * step
         else:
-            high += (n - 1) * s
-    return low, high + array.dtype.itemsize
+            high += (n - 1) * step
+    return low, high + dtype.itemsize
 
 
-def _refuse_overlap(out, name, other, other_name, same=False):
-    """ValueError when the result array touches an input; `same` allows the very same items."""
-    if same and out.address == other.address and out.dtype == other.dtype and (
-            out.shape[0] <= 1 or out.strides[0] == other.strides[0]):
-        return
-    low, high = _extent(out)
-    other_low, other_high = _extent(other)
-    if low >= high or other_low >= other_high or high <= other_low or other_high <= low:
-        return
-    # columns of one wider buffer may lie between each other without touching
-    if len(out.shape) == len(other.shape) == 2 and out.strides[0] == other.strides[0] > 0:
-        pitch = out.strides[0]
-        gap = (other.address - out.address) % pitch
-        if gap >= out.shape[1] * out.dtype.itemsize and gap + other.shape[1] * other.dtype.itemsize <= pitch:
-            return
-    raise ValueError("%s overlaps %s" % (name, other_name))
+def _refuse_overlaps(results, inputs, same=None):
+    """ValueError when a result array touches an input or another result; `same`: the input that a
+    result may be, item for item.  Both are lists of (tuple, name)."""
+    spans = [(*_extent(view), view, name) for view, name in results]
+    others = spans + [(*_extent(view), view, name) for view, name in inputs]
+    for at, (low, high, out, name) in enumerate(spans):
+        for other_low, other_high, other, other_name in others[at + 1:]:
+            if low < other_high and other_low < high and low < high and other_low < other_high and not (
+                    other is same and _same_items(out, other)) and not _beside(out, other):
+                raise ValueError("%s overlaps %s" % (name, other_name))
+
+
+def _same_items(out, other):
+    return out[0] == other[0] and out[3] == other[3] and (out[1][0] <= 1 or out[2][0] == other[2][0])
+
+
+def _beside(out, other):
+    """Columns of one wider buffer lie between each other without touching."""
+    if len(out[1]) == len(other[1]) == 2 and out[2][0] == other[2][0] > 0:
+        pitch = out[2][0]
+        gap = (other[0] - out[0]) % pitch
+        return gap >= out[1][1] * out[3].itemsize and gap + other[1][1] * other[3].itemsize <= pitch
+    return False
 
 
 def _number(value, name, low=None, high=None):
@@ -220,7 +258,7 @@ def _new(shape, dtype, stream, handle, name):
 
 
 def _result(obj, name, shape, dtype, stream, handle):
-    """(what the caller gets back, its _Array) for a result that may have been given."""
+    """(what the caller gets back, its tuple) for a result that may have been given."""
     if obj is None or obj is True:
         obj = _new(shape, dtype, stream, handle, name)
     return obj, _output(obj, name)
@@ -229,21 +267,24 @@ def _result(obj, name, shape, dtype, stream, handle):
 def _workspace(given, nbytes, handle):
     """(address, bytes, what keeps it alive)."""
     if given is not None:
-        array = _output(given, "workspace")
-        low, high = _extent(array)
+        view = _output(given, "workspace")
+        low, high = _extent(view)
         items = 1
-        for n in array.shape:
+        for n in view[1]:
             items *= n
-        if items * array.dtype.itemsize != high - low:
+        if items * view[3].itemsize != high - low:
             raise ValueError("workspace must be contiguous")
         if high - low < nbytes or low % 16:
             raise ValueError("workspace must hold %d bytes, aligned to 16" % nbytes)
-        return low, high - low, array.owner
+        return low, high - low, view[4]
     if not nbytes:
-        return 0, 0, None
+        return _NO_WORKSPACE
     if _capturing(handle):
         raise ValueError("a call that is captured into a graph needs a workspace of %d bytes" % nbytes)
     return devices.get_context().workspace(handle, nbytes)
+
+
+_NO_WORKSPACE = (0, 0, None)
 
 
 # ---- penalties, biases, masks --------------------------------------------------------------
@@ -257,8 +298,8 @@ def _per_row(value, name, rows, stream, number):
         if name == "repetition" and value <= 0:
             raise ValueError("repetition must be positive, got %r" % value)
         return 0, value, None
-    array = _as_vector(_input(value, name, stream, np.float32), name, rows, _FLOATS)
-    return array.address, number, array.owner
+    view = _as_vector(_input(value, name, stream, np.float32), name, rows, _FLOATS)
+    return view[0], number, view[4]
 
 
 def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, repetition=None, presence=None,
@@ -282,59 +323,66 @@ def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, 
     handle = _driver._stream_handle(stream)
     x = _input(logits, "logits", stream)
     in_stride = _as_rows(x, "logits")
-    rows, vocab = x.shape
+    shape, dtype = x[1], x[3]
+    rows, vocab = shape
     if (tokens is None) != (offsets is None):
         raise ValueError("tokens and offsets come together")
-    if tokens is None and any(v is not None for v in (prompt_lengths, repetition, presence, frequency)):
+    if tokens is None and not (prompt_lengths is repetition is presence is frequency is None):
         raise ValueError("penalties and prompt lengths need tokens and offsets")
-    if len({bias_tokens is None, bias_values is None, bias_offsets is None}) != 1:
+    if (bias_tokens is None) != (bias_values is None) or (bias_tokens is None) != (bias_offsets is None):
         raise ValueError("bias_tokens, bias_values and bias_offsets come together")
 
-    out, y = _result(out, "out", x.shape, x.dtype, stream, handle)
-    out_stride = _as_result_rows(y, "out", x.shape)
-    if y.dtype != x.dtype and y.dtype != _float32:
-        raise TypeError("out has dtype %s, expected %s or float32" % (y.dtype, x.dtype))
-    _refuse_overlap(y, "out", x, "logits", same=True)
+    out, y = _result(out, "out", shape, dtype, stream, handle)
+    out_stride = _as_result_rows(y, "out", shape)
+    if y[3] != dtype and y[3] != _float32:
+        raise TypeError("out has dtype %s, expected %s or float32" % (y[3], dtype))
+    _refuse_overlaps([(y, "out")], [(x, "logits")], same=x)
 
-    t = o = p = None
-    history = (0, 0, 0, 0, 4, 4, 4)
+    t = o = p = rep = pre = fre = bt = bo = bv = m = None        # alive until the launch is made
+    history, bias = _NO_HISTORY, _NO_BIAS
     if tokens is not None:
         t = _as_vector(_input(tokens, "tokens", stream), "tokens", None, _INTEGERS)
         o = _as_vector(_input(offsets, "offsets", stream), "offsets", rows + 1, _INTEGERS)
+        p = _NO_PROMPTS
         if prompt_lengths is not None:
             p = _as_vector(_input(prompt_lengths, "prompt_lengths", stream), "prompt_lengths", rows, _INTEGERS)
-        history = (t.address, o.address, p.address if p else 0, t.shape[0], t.dtype.itemsize, o.dtype.itemsize,
-                   p.dtype.itemsize if p else 4)
-    rep = _per_row(repetition, "repetition", rows, stream, 1.0)
-    pre = _per_row(presence, "presence", rows, stream, 0.0)
-    fre = _per_row(frequency, "frequency", rows, stream, 0.0)
-    bt = bo = bv = None
-    bias = (0, 0, 0, 0, 4, 4)
+        rep = _per_row(repetition, "repetition", rows, stream, 1.0)
+        pre = _per_row(presence, "presence", rows, stream, 0.0)
+        fre = _per_row(frequency, "frequency", rows, stream, 0.0)
+        history = (t[0], o[0], p[0], t[1][0], t[3].itemsize, o[3].itemsize, p[3].itemsize, rep[0], pre[0], fre[0],
+                   rep[1], pre[1], fre[1])
     if bias_tokens is not None:
         bt = _as_vector(_input(bias_tokens, "bias_tokens", stream), "bias_tokens", None, _INTEGERS)
-        bv = _as_vector(_input(bias_values, "bias_values", stream, np.float32), "bias_values", bt.shape[0], _FLOATS)
+        bv = _as_vector(_input(bias_values, "bias_values", stream, np.float32), "bias_values", bt[1][0], _FLOATS)
         bo = _as_vector(_input(bias_offsets, "bias_offsets", stream), "bias_offsets", rows + 1, _INTEGERS)
-        bias = (bt.address, bo.address, bv.address, bt.shape[0], bt.dtype.itemsize, bo.dtype.itemsize)
-    m, mask_stride = None, 0
+        bias = (bt[0], bo[0], bv[0], bt[1][0], bt[3].itemsize, bo[3].itemsize)
+    mask_address = mask_stride = 0
     if mask is not None:
         m = _input(mask, "mask", stream)
-        if m.dtype.kind not in "iu" or m.dtype.itemsize != 4:
-            raise TypeError("mask has dtype %s, expected 32-bit integers" % m.dtype)
-        if len(m.shape) not in (1, 2) or (len(m.shape) == 2 and m.shape[0] not in (1, rows)):
-            raise ValueError("mask has shape %s, expected one row of words or %d" % (m.shape, rows))
-        if m.shape[-1] * 32 < vocab:
-            raise ValueError("mask has %d words, %d entries need %d" % (m.shape[-1], vocab, -(-vocab // 32)))
-        if m.shape[-1] > 1 and m.strides[-1] != 4:
-            raise ValueError("the words of a mask must lie next to each other (strides %s)" % (m.strides,))
-        if len(m.shape) == 2 and m.shape[0] > 1:
-            mask_stride = m.strides[0]
+        mask_address, mask_shape, mask_strides, mask_dtype, _ = m
+        if mask_dtype.kind not in "iu" or mask_dtype.itemsize != 4:
+            raise TypeError("mask has dtype %s, expected 32-bit integers" % mask_dtype)
+        if len(mask_shape) not in (1, 2) or (len(mask_shape) == 2 and mask_shape[0] not in (1, rows)):
+            raise ValueError("mask has shape %s, expected one row of words or %d" % (tuple(mask_shape), rows))
+        words = mask_shape[-1]
+        if words * 32 < vocab:
+            raise ValueError("mask has %d words, %d entries need %d" % (words, vocab, -(-vocab // 32)))
+        if words > 1 and mask_strides[-1] != 4:
+            raise ValueError("the words of a mask must lie next to each other (strides %s)" % (mask_strides,))
+        if len(mask_shape) == 2 and mask_shape[0] > 1:
+            mask_stride = mask_strides[0]
 
     if rows and vocab:
         _driver.driver.nbh_logits_adjust(
-            _ADJUST.pack(_ADJUST.size, x.address, y.address, rows, vocab, in_stride, out_stride, _ROW_DTYPE[x.dtype],
-                         _ROW_DTYPE[y.dtype], *history, rep[0], pre[0], fre[0], rep[1], pre[1], fre[1], *bias,
-                         m.address if m else 0, mask_stride), handle or None)
+            _ADJUST.pack(_ADJUST_SIZE, x[0], y[0], rows, vocab, in_stride, out_stride, _ROW_DTYPE[dtype],
+                         _ROW_DTYPE[y[3]], *history, *bias, mask_address, mask_stride), handle or None)
     return out
+
+
+_ADJUST_SIZE = _ADJUST.size
+_NO_PROMPTS = (0, (0,), (4,), _int32, None)
+_NO_HISTORY = (0, 0, 0, 0, 4, 4, 4, 0, 0, 0, 1.0, 0.0, 0.0)
+_NO_BIAS = (0, 0, 0, 0, 4, 4)
 
 
 # ---- the largest entries of a row ----------------------------------------------------------
@@ -348,8 +396,9 @@ def _count(k, most):
 
 
 def _row_code(dtype):
-    dtype = _foreign_dtypes.get(dtype) or (np.dtype(dtype) if not str(dtype).startswith("torch.")
-                                           else _foreign_dtype(dtype))
+    if str(dtype).startswith("torch."):
+        dtype = _foreign_dtype(dtype)[0]
+    dtype = np.dtype(dtype)
     if dtype not in _ROW_DTYPE:
         raise TypeError("unsupported dtype %s" % dtype)
     return _ROW_DTYPE[dtype]
@@ -375,28 +424,28 @@ def top(logits, k, *, values=None, indices=None, lse=None, temperature=1.0, work
     handle = _driver._stream_handle(stream)
     x = _input(logits, "logits", stream)
     stride = _as_rows(x, "logits")
-    rows, vocab = x.shape
+    (rows, vocab), dtype = x[1], x[3]
     k = _count(k, min(vocab, MOST))
     temperature = _temperature(temperature)
     shape = (rows, k)
-    values, v = _result(values, "values", shape, x.dtype, stream, handle)
-    values_stride = _as_result_rows(v, "values", shape, (x.dtype,))
-    _refuse_overlap(v, "values", x, "logits")
+    values, v = _result(values, "values", shape, dtype, stream, handle)
+    values_stride = _as_result_rows(v, "values", shape, (dtype,))
     indices, i = _result(indices, "indices", shape, _int32, stream, handle)
     indices_stride = _as_result_rows(i, "indices", shape, (_int32,))
-    _refuse_overlap(i, "indices", x, "logits")
-    z = None
-    if lse is not None and lse is not False:
+    results, lse_address = [(v, "values"), (i, "indices")], None
+    wanted = lse is not None and lse is not False
+    if wanted:
         lse, z = _result(lse, "lse", (rows,), _float32, stream, handle)
         _as_vector(z, "lse", rows, _FLOATS)
-        _refuse_overlap(z, "lse", x, "logits")
-    code = _ROW_DTYPE[x.dtype]
+        lse_address = z[0]
+        results.append((z, "lse"))
+    _refuse_overlaps(results, [(x, "logits")])
+    code = _ROW_DTYPE[dtype]
     if rows:
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_top_workspace(rows, vocab, k, code), handle)
-        _driver.driver.nbh_rows_top(x.address, rows, vocab, stride, code, k, v.address, values_stride, i.address,
-                                    indices_stride, z.address if z else None, temperature, space[0] or None,
-                                    space[1], handle or None)
-    return (values, indices) if z is None else (values, indices, lse)
+        _driver.driver.nbh_rows_top(x[0], rows, vocab, stride, code, k, v[0], values_stride, i[0], indices_stride,
+                                    lse_address, temperature, space[0] or None, space[1], handle or None)
+    return (values, indices, lse) if wanted else (values, indices)
 
 
 # ---- distillation --------------------------------------------------------------------------
@@ -413,66 +462,66 @@ def _distill(what, grad_loss, student, values, indices, temperature, teacher_lse
     handle = _driver._stream_handle(stream)
     x = _input(student, "student", stream)
     stride = _as_rows(x, "student")
-    rows, vocab = x.shape
+    shape, dtype = x[1], x[3]
+    rows, vocab = shape
     v = _input(values, "values", stream)
     values_stride = _as_rows(v, "values")
     i = _input(indices, "indices", stream)
-    indices_stride = _as_rows(i, "indices", v.shape, _INTEGERS)
-    if v.shape[0] != rows:
-        raise ValueError("values has %d rows, student has %d" % (v.shape[0], rows))
-    k = v.shape[1]
+    indices_stride = _as_rows(i, "indices", v[1], _INTEGERS)
+    if v[1][0] != rows:
+        raise ValueError("values has %d rows, student has %d" % (v[1][0], rows))
+    k = v[1][1]
     if k > MOST:
         raise ValueError("a row of values may hold %d entries, got %d" % (MOST, k))
     temperature = _temperature(temperature)
-    t = g = None
+    inputs, results = [(x, "student"), (v, "values"), (i, "indices")], []
+    teacher_address = grad_address = grad_stride = loss_address = out_address = out_stride = 0
+    grad_value = 0.0
     if teacher_lse is not None:
         t = _as_vector(_input(teacher_lse, "teacher_lse", stream, np.float32), "teacher_lse", rows, _FLOATS)
-    g_stride, g_value = 0, 0.0
+        teacher_address = t[0]
+        inputs.append((t, "teacher_lse"))
     if what & _GRAD:
         if _is_number(grad_loss):
-            g_value = _number(grad_loss, "grad_loss")
+            grad_value = _number(grad_loss, "grad_loss")
         else:
             g = _input(grad_loss, "grad_loss", stream, np.float32)
-            if g.shape != (rows,):
-                raise ValueError("grad_loss has shape %s, expected (%d,)" % (g.shape, rows))
-            if g.dtype != _float32:
-                raise TypeError("grad_loss has unsupported dtype %s" % g.dtype)
-            g_stride = g.strides[0]
-            if g.address % 4 or g_stride % 4:
+            grad_address, grad_shape, strides, grad_dtype, _ = g
+            if len(grad_shape) != 1 or grad_shape[0] != rows:
+                raise ValueError("grad_loss has shape %s, expected (%d,)" % (tuple(grad_shape), rows))
+            if grad_dtype != _float32:
+                raise TypeError("grad_loss has unsupported dtype %s" % grad_dtype)
+            grad_stride = strides[0]
+            if grad_address % 4 or grad_stride % 4:
                 raise ValueError("grad_loss is not aligned to its item size")
-
-    small = [(v, "values"), (i, "indices")] + ([(t, "teacher_lse")] if t else []) + ([(g, "grad_loss")] if g else [])
-    l = z = y = None
+            inputs.append((g, "grad_loss"))
     if what & _LOSS:
         loss, l = _result(loss, "loss", (rows,), _float32, stream, handle)
-        _as_vector(l, "loss", rows, _FLOATS)
+        loss_address = _as_vector(l, "loss", rows, _FLOATS)[0]
         lse, z = _result(lse, "lse", (rows,), _float32, stream, handle)
         _as_vector(z, "lse", rows, _FLOATS)
-        for other in small + [(x, "student"), (z, "lse")]:
-            _refuse_overlap(l, "loss", *other)
-        for other in small + [(x, "student")]:
-            _refuse_overlap(z, "lse", *other)
+        results += [(l, "loss"), (z, "lse")]
     else:
         z = _as_vector(_input(lse, "lse", stream, np.float32), "lse", rows, _FLOATS)
-        small.append((z, "lse"))
-    out_stride = 0
+        inputs.append((z, "lse"))
     if what & _GRAD:
-        out, y = _result(out, "out", x.shape, x.dtype, stream, handle)
-        out_stride = _as_result_rows(y, "out", x.shape, (x.dtype,))
-        _refuse_overlap(y, "out", x, "student", same=True)
-        for other in small + ([(l, "loss"), (z, "lse")] if what & _LOSS else []):
-            _refuse_overlap(y, "out", *other)
+        out, y = _result(out, "out", shape, dtype, stream, handle)
+        out_address, out_stride = y[0], _as_result_rows(y, "out", shape, (dtype,))
+        results.append((y, "out"))
+    _refuse_overlaps(results, inputs, same=x)
 
     if rows:
-        code = _ROW_DTYPE[x.dtype]
+        code = _ROW_DTYPE[dtype]
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_distill_workspace(rows, vocab, k, code, what), handle)
         _driver.driver.nbh_rows_distill(
-            _DISTILL.pack(_DISTILL.size, what, x.address, rows, vocab, stride, code, v.address, i.address, k,
-                          values_stride, _ROW_DTYPE[v.dtype], indices_stride, i.dtype.itemsize,
-                          t.address if t else 0, g.address if g else 0, g_stride, g_value, temperature,
-                          l.address if l else 0, z.address, y.address if y else 0, out_stride, space[0], space[1]),
+            _DISTILL.pack(_DISTILL_SIZE, what, x[0], rows, vocab, stride, code, v[0], i[0], k, values_stride,
+                          _ROW_DTYPE[v[3]], indices_stride, i[3].itemsize, teacher_address, grad_address, grad_stride,
+                          grad_value, temperature, loss_address, z[0], out_address, out_stride, space[0], space[1]),
             handle or None)
     return loss, lse, out
+
+
+_DISTILL_SIZE = _DISTILL.size
 
 
 def distill_loss(student, values, indices, *, temperature=1.0, teacher_lse=None, loss=None, lse=None, workspace=None,

@@ -139,14 +139,18 @@ def test_adjust_refusals(fake_gpu):
 
 def test_columns_beside_each_other_do_not_overlap():
     def array(start, n, pitch=100, rows=3):
-        return logits._Array(4096 + 4 * start, (rows, n), (4 * pitch, 4), np.dtype(np.float32), None)
-    logits._refuse_overlap(array(0, 40), "out", array(40, 60), "logits")
-    logits._refuse_overlap(array(40, 60), "out", array(0, 40), "logits")
+        return 4096 + 4 * start, (rows, n), (4 * pitch, 4), np.dtype(np.float32), None
+    def check(one, other, same=None):
+        logits._refuse_overlaps([(one, "out")], [(other, "logits")], same=same)
+    check(array(0, 40), array(40, 60))
+    check(array(40, 60), array(0, 40))
     for start, n in ((39, 10), (0, 40), (30, 5), (90, 20)):
-        with pytest.raises(ValueError):
-            logits._refuse_overlap(array(0, 40), "out", array(start, n, rows=4), "logits", same=True) \
-                if (start, n) != (0, 40) else logits._refuse_overlap(array(0, 40), "out", array(0, 40), "logits")
-    logits._refuse_overlap(array(0, 40), "out", array(0, 40), "logits", same=True)
+        with pytest.raises(ValueError, match="out overlaps logits"):
+            check(array(0, 40), array(start, n, rows=4))
+    x = array(0, 40)
+    check(array(0, 40), x, same=x)
+    with pytest.raises(ValueError):
+        check(array(0, 40, pitch=99), x, same=x)
 
 
 def test_top_refusals(fake_gpu):
