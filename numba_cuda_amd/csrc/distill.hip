@@ -4,19 +4,31 @@
 //   loss = sum p_j (log p_j - (s[i_j] / T - lse))
 //   grad[v] = grad_loss / T * (P exp(s[v] / T - lse) - sum over i_j = v of p_j)
 //
-// One workgroup per row: the teacher's entries go to LDS, one pass over the row gives its maximum and
-// sum together, the second writes the gradient as a * 2^((s - m) * c) for every entry, and behind a
-// barrier the few entries the teacher names are written again with their p_j taken off.  The row's second
-// reading comes out of the caches.  Few rows are split over workgroups: a launch for the statistics of the
-// stretches, then one that joins them and works on the stretches.
+// One workgroup per row: its first wavefront brings the teacher's entries to LDS while the others begin
+// the pass over the row that gives its maximum and sum together; a second pass, backwards, so that it finds
+// the end of the first in the caches, writes the gradient as a * 2^((s - m) * c) for every entry, and behind
+// a barrier the few entries the teacher names are written again with their p_j taken off.  Few rows are
+// split over workgroups: a launch for the statistics of the stretches, then one that joins them and works
+// on the stretches.  A large gradient by itself is a copy with arithmetic: a launch prepares two numbers
+// for each row, small workgroups in memory order do the copy, a last launch writes the named entries.
 #include "rows.h"
 
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWaves = kThreads / 64;
+constexpr int kStatsThreads = 256;
 constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f;       // log2(e) and its rounding
 constexpr float kLn2 = 0.693147180559945309f;
+
+// exp(s / T - lse) P grad_loss / T = whole * 2^(s * scale - peak * scale) for a row; 0 where `zero`.
+struct Plan {
+    float peak, whole;
+    int zero, unused;
+};
+// An entry of the gradient that the teacher names: its index (-1: none) and value.
+struct Named {
+    int32_t index;
+    float value;
+};
 
 struct Distill {
     const char *student;
@@ -33,54 +45,42 @@ struct Distill {
     int64_t grad_stride;
     nbh_softmax *parts;                  // per row and stretch
     float *targets;                      // per row: the student's values at the teacher's k indices
+    Plan *plans;                         // per row
+    Named *named;                        // per row and teacher's entry
+    int tiles;
 };
 
 template <typename E>
-__global__ __launch_bounds__(kThreads) void distill_stats(Distill a)
+__global__ __launch_bounds__(kStatsThreads) void distill_stats(Distill a)
 {
-    __shared__ nbh_softmax room[kWaves];
+    constexpr int T = kStatsThreads;
+    __shared__ nbh_softmax room[T / 64];
     const int64_t row = a.row0 + blockIdx.x / a.splits;
     const int split = blockIdx.x % a.splits;
     const typename E::item *in = reinterpret_cast<const typename E::item *>(a.student + row * a.stride);
     const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
-    const nbh_softmax stats =
-        nbh_softmax_group<kThreads>(nbh_row_stats<E, kThreads, false>(in, begin, end, a.scale), a.scale, room);
+    const nbh_softmax stats = nbh_softmax_group<T>(nbh_row_stats<E, T, false>(in, begin, end, a.scale), a.scale, room);
     if (threadIdx.x == 0)
         a.parts[(row - a.row0) * a.splits + split] = stats;
     // The loss needs these of the whole row, and the gradient may be written over the row while another
     // stretch's workgroup still works on the loss: they are set aside.
     if (split == 0)
-        for (int j = threadIdx.x; j < a.k; j += kThreads) {
+        for (int j = threadIdx.x; j < a.k; j += T) {
             const int64_t at = nbh_row_int(a.indices + row * a.indices_stride, a.index_bytes, j);
             a.targets[(row - a.row0) * a.k + j] = at >= 0 && at < a.vocab ? E::get(in[at]) : 0.0f;
         }
 }
 
-// The sum of x over the workgroup, in every lane; the barriers also order what was written to LDS before.
-__device__ __forceinline__ float group_add(float x, float *room)
+__device__ __forceinline__ float wave_add(float x)
 {
     for (int step = 32; step; step >>= 1)
         x += __shfl_xor(x, step);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        room[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = room[0];
-    for (int w = 1; w < kWaves; ++w)
-        x += room[w];
     return x;
 }
-__device__ __forceinline__ float group_max(float x, float *room)
+__device__ __forceinline__ float wave_max(float x)
 {
     for (int step = 32; step; step >>= 1)
         x = fmaxf(x, __shfl_xor(x, step));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-        room[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = room[0];
-    for (int w = 1; w < kWaves; ++w)
-        x = fmaxf(x, room[w]);
     return x;
 }
 
@@ -97,21 +97,181 @@ __device__ __forceinline__ float teacher_value(const Distill &a, int64_t row, in
     }
 }
 
-// What one launch of the row kernel does
-constexpr int kLoss = 1, kGrad = 2, kParts = 4;      // kParts: statistics come from distill_stats
+// What a launch does; kParts: the statistics come from distill_stats.
+constexpr int kLoss = 1, kGrad = 2, kParts = 4;
 
+// The teacher's entries of a row in LDS: index (-1: absent), p, log p, and the student's value there.
+struct Teacher {
+    int32_t *index;
+    float *p, *log_p, *student;
+    int32_t *table;                      // at least 2 k slots, for the search for repeated indices
+    float mass;
+    int some, repeated;
+
+    static __host__ __device__ int slots(int k)
+    {
+        int n = 2;
+        while (n < 2 * k)
+            n *= 2;
+        return n;
+    }
+    static size_t bytes(int k) { return (size_t)k * 16 + (size_t)slots(k) * 4; }
+    __device__ void place(char *lds, int k)
+    {
+        index = reinterpret_cast<int32_t *>(lds);
+        p = reinterpret_cast<float *>(index + k);
+        log_p = p + k;
+        student = log_p + k;
+        table = reinterpret_cast<int32_t *>(student + k);
+    }
+};
+
+// One wavefront's work: no barriers, its LDS accesses are in order.  `begin` .. `end`: the part of the row
+// whose values are wanted (elsewhere another workgroup may be writing the gradient over them already).
 template <typename E, int WHAT>
-__global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
+__device__ void load_teacher(const Distill &a, int64_t row, int64_t begin, int64_t end, Teacher &t)
+{
+    const typename E::item *in = reinterpret_cast<const typename E::item *>(a.student + row * a.stride);
+    const int lane = threadIdx.x & 63;
+    const int slots = Teacher::slots(a.k);
+    if (WHAT & kGrad)
+        for (int i = lane; i < slots; i += 64)
+            t.table[i] = -1;
+    float peak = -FLT_MAX;
+    int some = 0;
+    for (int j = lane; j < a.k; j += 64) {
+        const int64_t at = nbh_row_int(a.indices + row * a.indices_stride, a.index_bytes, j);
+        const float value = teacher_value(a, row, j);
+        const bool present = at >= 0 && at < a.vocab && value != -INFINITY;
+        t.index[j] = present ? (int32_t)at : -1;
+        t.log_p[j] = value;
+        if (present) {
+            t.student[j] = WHAT & kParts                ? a.targets[(row - a.row0) * a.k + j]
+                           : at >= begin && at < end ? E::get(in[at])
+                                                        : 0.0f;
+            peak = fmaxf(peak, fminf(value, FLT_MAX));
+            some = 1;
+        }
+    }
+    // p = exp(value / T - norm), or relative to the peak and then divided by the sum
+    const float norm = a.teacher_lse ? a.teacher_lse[row] : 0.0f;
+    if (!a.teacher_lse)
+        peak = wave_max(peak);
+    float sum = 0.0f;
+    for (int j = lane; j < a.k; j += 64) {
+        const float z = a.teacher_lse ? t.log_p[j] / a.temperature - norm : (t.log_p[j] - peak) / a.temperature;
+        t.log_p[j] = z;
+        t.p[j] = t.index[j] >= 0 ? expf(z) : 0.0f;
+        sum += t.p[j];
+    }
+    sum = wave_add(sum);
+    t.mass = sum;
+    if (!a.teacher_lse) {
+        const float log_sum = logf(sum);
+        float mass = 0.0f;
+        for (int j = lane; j < a.k; j += 64) {
+            t.log_p[j] -= log_sum;
+            t.p[j] = t.index[j] >= 0 ? t.p[j] / sum : 0.0f;
+            mass += t.p[j];
+        }
+        t.mass = wave_add(mass);
+    }
+    t.some = __any(some);
+    int repeated = 0;
+    if (WHAT & kGrad)
+        for (int j = lane; j < a.k; j += 64)
+            if (t.index[j] >= 0) {
+                uint32_t slot = (uint32_t)t.index[j] * 2654435761u;
+                for (int tries = 0; tries < slots; ++tries, ++slot) {
+                    const int32_t was = atomicCAS(&t.table[slot & (slots - 1)], -1, t.index[j]);
+                    repeated |= was == t.index[j];
+                    if (was == -1 || was == t.index[j])
+                        break;
+                }
+            }
+    t.repeated = __any(repeated);
+}
+
+// The student's side of a row: q(v) = base * 2^(s scale - peak scale).
+struct Student {
+    float peak, base, log_sum;           // log_sum: log2 of the sum relative to the peak
+};
+__device__ __forceinline__ Student student_of(nbh_softmax stats)
+{
+    return {stats.peak == -INFINITY ? 0.0f : stats.peak, stats.sum == 0.0f ? 0.0f : 1.0f / stats.sum, log2f(stats.sum)};
+}
+__device__ __forceinline__ Student student_of_lse(const Distill &a, float lse)
+{
+    // T * lse rounded to float32 takes the place of the peak; what the roundings of it, of its product
+    // with the scale, and of the scale itself take off goes into the factor.
+    const float peak = lse * a.temperature, product = peak * a.scale;
+    if (lse == -INFINITY)
+        return {0.0f, 0.0f, 0.0f};
+    if (nbh_softmax_near(product)) {
+        const float high = lse * kLog2e, low = fmaf(lse, kLog2e, -high) + lse * kLog2eRest;
+        return {peak, exp2f((product - high) - low + peak * a.scale_rest), 0.0f};
+    }
+    const float rest = __builtin_isfinite(peak) ? fmaf(lse, a.temperature, -peak) : 0.0f;
+    return {peak, expf(-rest / a.temperature), 0.0f};
+}
+
+// One wavefront's work.
+__device__ float loss_of(const Distill &a, const Teacher &t, Student s)
+{
+    const float product = s.peak * a.scale;
+    float loss = 0.0f;
+    for (int j = threadIdx.x & 63; j < a.k; j += 64)
+        if (t.index[j] >= 0 && t.p[j] != 0.0f) {
+            const float x = t.student[j];
+            float log_q = x;
+            if (x != -INFINITY)
+                log_q = nbh_softmax_near(product) && fabsf(x) < 1e30f
+                            ? (fmaf(x, a.scale, -product) - s.log_sum) * kLn2
+                            : (x - s.peak) / a.temperature - s.log_sum * kLn2;
+            loss += t.p[j] * (t.log_p[j] - log_q);
+        }
+    loss = wave_add(loss);
+    return t.some ? loss : 0.0f;
+}
+
+__device__ __forceinline__ float factor_of(const Distill &a, int64_t row)
+{
+    const float grad_loss =
+        a.grad_loss ? *reinterpret_cast<const float *>((const char *)a.grad_loss + row * a.grad_loss_stride)
+                    : a.grad_loss_value;
+    return grad_loss / a.temperature;
+}
+
+// The gradient at the teacher's entry j; index -1 if there is none, or an earlier entry of the same index
+// answers for it.
+__device__ __forceinline__ Named named_of(const Distill &a, const Teacher &t, int j, Student s, float whole,
+                                          float factor)
+{
+    const int32_t index = t.index[j];
+    if (index < 0)
+        return {-1, 0.0f};
+    float own = t.p[j];
+    if (t.repeated) {                    // the first of them takes all their shares, in order
+        for (int i = 0; i < j; ++i)
+            if (t.index[i] == index)
+                return {-1, 0.0f};
+        for (int i = j + 1; i < a.k; ++i)
+            if (t.index[i] == index)
+                own += t.p[i];
+    }
+    return {index, whole * nbh_softmax_term(t.student[j], s.peak, a.scale) - factor * own};
+}
+
+template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void distill_rows(Distill a)
 {
     typedef typename E::item item;
     constexpr int kItems = E::items;
-    extern __shared__ char lds[];        // index, p and log p, and the table that finds repeated indices
-    __shared__ nbh_softmax room[kWaves];
-    __shared__ float add_room[kWaves];
-    __shared__ int repeated;
-    int32_t *const index = reinterpret_cast<int32_t *>(lds);
-    float *const p = reinterpret_cast<float *>(index + a.k), *const log_p = p + a.k;
-    int32_t *const table = reinterpret_cast<int32_t *>(log_p + a.k);
+    extern __shared__ char lds[];
+    __shared__ nbh_softmax room[T / 64];
+    __shared__ float mass;
+    __shared__ int some, repeated;
+    Teacher teacher;
+    teacher.place(lds, a.k);
 
     // the loss alone takes one workgroup per row, whatever the statistics took
     constexpr bool kWhole = WHAT == (kLoss | kParts);
@@ -120,231 +280,183 @@ __global__ __launch_bounds__(kThreads) void distill_rows(Distill a)
     const item *in = reinterpret_cast<const item *>(a.student + row * a.stride);
     const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
 
-    // -- the teacher's entries
-    float peak = -FLT_MAX;
-    int some = 0;
-    for (int j = threadIdx.x; j < a.k; j += kThreads) {
-        const int64_t at = nbh_row_int(a.indices + row * a.indices_stride, a.index_bytes, j);
-        const float t = teacher_value(a, row, j);
-        const bool present = at >= 0 && at < a.vocab && t != -INFINITY;
-        index[j] = present ? (int32_t)at : -1;
-        log_p[j] = t;
-        if (present) {
-            peak = fmaxf(peak, fminf(t, FLT_MAX));
-            some = 1;
+    if (threadIdx.x < 64) {
+        load_teacher<E, WHAT>(a, row, WHAT & kLoss ? 0 : begin, WHAT & kLoss ? a.vocab : end, teacher);
+        if (threadIdx.x == 0) {
+            mass = teacher.mass;
+            some = teacher.some;
+            repeated = teacher.repeated;
         }
     }
-    float mass = 0.0f;
-    if (a.teacher_lse) {
-        const float norm = a.teacher_lse[row];
-        for (int j = threadIdx.x; j < a.k; j += kThreads) {
-            log_p[j] = log_p[j] / a.temperature - norm;
-            p[j] = index[j] >= 0 ? expf(log_p[j]) : 0.0f;
-            mass += p[j];
-        }
-        mass = group_add(mass, add_room);
-    } else {
-        peak = group_max(peak, add_room);
-        float sum = 0.0f;
-        for (int j = threadIdx.x; j < a.k; j += kThreads) {
-            log_p[j] = (log_p[j] - peak) / a.temperature;
-            p[j] = index[j] >= 0 ? expf(log_p[j]) : 0.0f;
-            sum += p[j];
-        }
-        sum = group_add(sum, add_room);
-        const float norm = logf(sum);
-        for (int j = threadIdx.x; j < a.k; j += kThreads) {
-            log_p[j] -= norm;
-            p[j] = index[j] >= 0 ? p[j] / sum : 0.0f;
-            mass += p[j];
-        }
-        mass = group_add(mass, add_room);
-    }
-    some = __syncthreads_or(some);
-
-    // -- the student's statistics: exp(s / T - lse) = base * 2^(s * scale - peak * scale)
-    float peak_s, base, log_sum = 0.0f;
+    Student student;
     if (WHAT & kLoss) {
         nbh_softmax stats;
         if (WHAT & kParts) {
             stats = a.parts[(row - a.row0) * a.splits];
             for (int s = 1; s < a.splits; ++s)
                 stats = nbh_softmax_join(stats, a.parts[(row - a.row0) * a.splits + s], a.scale);
+            __syncthreads();
         } else {
-            stats = nbh_softmax_group<kThreads>(nbh_row_stats<E, kThreads, false>(in, 0, a.vocab, a.scale), a.scale,
-                                                room);
+            stats = nbh_softmax_group<T>(nbh_row_stats<E, T, false>(in, 0, a.vocab, a.scale), a.scale, room);
         }
-        peak_s = stats.peak == -INFINITY ? 0.0f : stats.peak;
-        base = stats.sum == 0.0f ? 0.0f : 1.0f / stats.sum;
-        log_sum = log2f(stats.sum);
+        student = student_of(stats);
         if (a.lse && split == 0 && threadIdx.x == 0)
             a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
-    } else {
-        const float lse = a.lse[row];
-        // T * lse rounded to float32 takes the place of the largest value; what the roundings of it, of
-        // its product with the scale, and of the scale itself take off goes into the factor.
-        peak_s = lse * a.temperature;
-        const float product = peak_s * a.scale;
-        if (nbh_softmax_near(product)) {
-            const float high = lse * kLog2e, low = fmaf(lse, kLog2e, -high) + lse * kLog2eRest;
-            base = exp2f((product - high) - low + peak_s * a.scale_rest);
-        } else {
-            const float rest = __builtin_isfinite(peak_s) ? fmaf(lse, a.temperature, -peak_s) : 0.0f;
-            base = expf(-rest / a.temperature);
+        if (split == 0 && threadIdx.x < 64) {
+            const float loss = loss_of(a, teacher, student);
+            if (threadIdx.x == 0)
+                a.loss[row] = loss;
         }
-        if (lse == -INFINITY)
-            peak_s = base = 0.0f;
-    }
-    const float product = peak_s * a.scale;
-    const bool near = nbh_softmax_near(product);
-
-    // -- loss
-    if ((WHAT & kLoss) && split == 0) {
-        float loss = 0.0f;
-        for (int j = threadIdx.x; j < a.k; j += kThreads)
-            if (index[j] >= 0 && p[j] != 0.0f) {
-                const float s = WHAT & kParts ? a.targets[(row - a.row0) * a.k + j] : E::get(in[index[j]]);
-                float log_q = s;
-                if (s != -INFINITY)
-                    log_q = near && fabsf(s) < 1e30f
-                                ? (fmaf(s, a.scale, -product) - log_sum) * kLn2
-                                : (s - peak_s) / a.temperature - log_sum * kLn2;
-                loss += p[j] * (log_p[j] - log_q);
-            }
-        loss = group_add(loss, add_room);
-        if (threadIdx.x == 0)
-            a.loss[row] = some ? loss : 0.0f;
+    } else {
+        student = student_of_lse(a, a.lse[row]);
+        __syncthreads();
     }
     if (!(WHAT & kGrad))
         return;
 
-    // -- gradient
     item *out = reinterpret_cast<item *>(a.grad + row * a.grad_stride);
-    const float factor =
-        (a.grad_loss ? *reinterpret_cast<const float *>((const char *)a.grad_loss + row * a.grad_loss_stride)
-                     : a.grad_loss_value) /
-        a.temperature;
+    const float factor = factor_of(a, row);
     if (!some || factor == 0.0f) {
         float zero[kItems] = {};
-        for (int64_t at = begin + threadIdx.x * kItems; at < end; at += kThreads * kItems)
+        for (int64_t at = begin + threadIdx.x * kItems; at < end; at += T * kItems)
             nbh_row_store<E, true>(out, at, end, zero);
         return;
     }
-    // which of the teacher's indices occur more than once (none, as a rule): a table of at least 2 k slots
-    int slots = 2;
-    while (slots < 2 * a.k)
-        slots *= 2;
-    for (int i = threadIdx.x; i < slots; i += kThreads)
-        table[i] = -1;
-    if (threadIdx.x == 0)
-        repeated = 0;
-    __syncthreads();
-    for (int j = threadIdx.x; j < a.k; j += kThreads)
-        if (index[j] >= 0) {
-            uint32_t slot = (uint32_t)index[j] * 2654435761u;
-            for (int tries = 0; tries < slots; ++tries, ++slot) {
-                const int32_t was = atomicCAS(&table[slot & (slots - 1)], -1, index[j]);
-                if (was == index[j])
-                    repeated = 1;
-                if (was == -1 || was == index[j])
-                    break;
-            }
-        }
-    __syncthreads();
-    // the student's values at the teacher's entries, before they are written over
-    const float whole = factor * mass * base;
-    for (int j = threadIdx.x; j < a.k; j += kThreads) {
-        if (index[j] < begin || index[j] >= end)
-            continue;
-        float own = p[j];
-        if (repeated) {                  // the first of them takes all their shares, in order
-            bool first = true;
-            for (int i = 0; i < j && first; ++i)
-                first = index[i] != index[j];
-            for (int i = j + 1; i < a.k && first; ++i)
-                if (index[i] == index[j])
-                    own += p[i];
-            if (!first) {
-                log_p[j] = 0.0f;
-                continue;
-            }
-        }
-        const float s = E::get(in[index[j]]);
-        log_p[j] = whole * nbh_softmax_term(s, peak_s, a.scale) - factor * own;
-    }
-    __syncthreads();
-    nbh_row_stream<E, kThreads, false, true>(in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
+    const float whole = factor * mass * student.base, product = student.peak * a.scale;
+    const bool near = nbh_softmax_near(product);
+    nbh_row_stream<E, T, true, true>(
+        in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < kNbhAhead; ++j) {
-            float f[kItems];
-            E::unpack(raw[j], f);
-            if (near) {
+            for (int j = 0; j < kNbhAhead; ++j) {
+                float f[kItems];
+                E::unpack(raw[j], f);
+                if (near) {
 #pragma unroll
-                for (int i = 0; i < kItems; ++i)
-                    f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
-            } else {
-                for (int i = 0; i < kItems; ++i)
-                    f[i] = whole * nbh_exp2((f[i] - peak_s) * a.scale);
+                    for (int i = 0; i < kItems; ++i)
+                        f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+                } else {
+                    for (int i = 0; i < kItems; ++i)
+                        f[i] = whole * nbh_exp2((f[i] - student.peak) * a.scale);
+                }
+                nbh_row_store<E, true>(out, at + (j * T + threadIdx.x) * kItems, end, f);
             }
-            nbh_row_store<E, true>(out, at + (j * kThreads + threadIdx.x) * kItems, end, f);
-        }
-    });
+        });
     __syncthreads();
-    for (int j = threadIdx.x; j < a.k; j += kThreads) {
-        if (index[j] < begin || index[j] >= end)
-            continue;
-        if (repeated) {
-            bool first = true;
-            for (int i = 0; i < j && first; ++i)
-                first = index[i] != index[j];
-            if (!first)
-                continue;
+    teacher.repeated = repeated;
+    for (int j = threadIdx.x; j < a.k; j += T)
+        if (teacher.index[j] >= begin && teacher.index[j] < end) {
+            const Named n = named_of(a, teacher, j, student, whole, factor);
+            if (n.index >= 0)
+                out[n.index] = E::put(n.value);
         }
-        out[index[j]] = E::put(log_p[j]);
-    }
 }
 
-// Stretches of a row: one workgroup per row from 1024 rows on, else workgroups for four per compute unit.
-struct Split {
+// The gradient in three launches.  First: a wavefront per row.
+template <typename E> __global__ __launch_bounds__(64) void distill_plan(Distill a)
+{
+    extern __shared__ char lds[];
+    const int64_t row = a.row0 + blockIdx.x;
+    Teacher teacher;
+    teacher.place(lds, a.k);
+    load_teacher<E, kGrad>(a, row, 0, a.vocab, teacher);
+    const Student student = student_of_lse(a, a.lse[row]);
+    const float factor = factor_of(a, row);
+    const bool zero = !teacher.some || factor == 0.0f;
+    const float whole = factor * teacher.mass * student.base;
+    if (threadIdx.x == 0)
+        a.plans[row - a.row0] = {student.peak, whole, zero, 0};
+    for (int j = threadIdx.x; j < a.k; j += 64)
+        a.named[(row - a.row0) * a.k + j] = zero ? Named{-1, 0.0f} : named_of(a, teacher, j, student, whole, factor);
+}
+// Second: 4 KiB of a row per workgroup, in the order of memory.
+template <typename E> __global__ __launch_bounds__(256) void distill_flat(Distill a)
+{
+    typedef typename E::item item;
+    constexpr int kItems = E::items;
+    const int64_t row = blockIdx.x / a.tiles;
+    const int64_t at = ((int64_t)(blockIdx.x % a.tiles) * 256 + threadIdx.x) * kItems;
+    if (at >= a.vocab)
+        return;
+    const item *in = reinterpret_cast<const item *>(a.student + (a.row0 + row) * a.stride);
+    item *out = reinterpret_cast<item *>(a.grad + (a.row0 + row) * a.grad_stride);
+    float f[kItems];
+    nbh_row_load<E, true>(in, at, a.vocab, 0.0f, f);
+    const Plan plan = a.plans[row];
+    const float product = plan.peak * a.scale;
+    if (plan.zero) {
+        for (int i = 0; i < kItems; ++i)
+            f[i] = 0.0f;
+    } else if (nbh_softmax_near(product)) {
+        for (int i = 0; i < kItems; ++i)
+            f[i] = plan.whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+    } else {
+        for (int i = 0; i < kItems; ++i)
+            f[i] = plan.whole * nbh_exp2((f[i] - plan.peak) * a.scale);
+    }
+    nbh_row_store<E, true>(out, at, a.vocab, f);
+}
+// Third: a lane per entry the teacher names.
+template <typename E> __global__ __launch_bounds__(256) void distill_named(Distill a, int64_t rows)
+{
+    const int64_t i = blockIdx.x * (int64_t)256 + threadIdx.x;
+    if (i >= rows * a.k)
+        return;
+    const Named n = a.named[i];
+    if (n.index >= 0)
+        reinterpret_cast<typename E::item *>(a.grad + (a.row0 + i / a.k) * a.grad_stride)[n.index] = E::put(n.value);
+}
+
+// How a call is spread.
+//   splits, slice   stretches of a row: one workgroup per row from 1024 rows on, else workgroups for four per
+//                   compute unit
+//   flat            the gradient by itself in three launches, where its rows hold 64 MiB or more
+struct Spread {
+    bool flat;
     int splits;
     int64_t slice;
 };
-Split split_of(int64_t rows, int64_t vocab, int dtype)
+Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what)
 {
-    const int64_t chunk = (int64_t)kThreads * kNbhAhead * (dtype == NBH_ROW_F32 ? 4 : 8);
+    const int64_t items = dtype == NBH_ROW_F32 ? 4 : 8;
+    if (what == kGrad && rows * vocab >= ((int64_t)64 << 20) / 16 * items)
+        return {true, 1, vocab};
+    const int64_t chunk = kStatsThreads * kNbhAhead * items;
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
         splits = chunks;
     const int64_t each = (chunks + splits - 1) / splits;
-    return {(int)((chunks + each - 1) / each), each * chunk};
+    return {false, (int)((chunks + each - 1) / each), each * chunk};
 }
 
 template <typename E>
-int launch_distill(Distill a, int64_t rows, int what, hipStream_t stream)
+int launch_distill(Distill a, bool flat, int64_t rows, int what, hipStream_t stream)
 {
-    int slots = 2;
-    while (slots < 2 * a.k)
-        slots *= 2;
-    const size_t bytes = (size_t)a.k * 12 + (size_t)slots * 4;
-    const int64_t most = NBH_ROW_MOST_GROUPS / a.splits;
+    const size_t bytes = Teacher::bytes(a.k);
+    a.tiles = (int)((a.vocab + 256 * E::items - 1) / (256 * E::items));
+    const int64_t most = NBH_ROW_MOST_GROUPS / (flat ? a.tiles : a.splits);
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
-        const dim3 block(kThreads);
-        dim3 grid((unsigned)(now * a.splits));
-        if (what == kGrad) {
-            distill_rows<E, kGrad><<<grid, block, bytes, stream>>>(a);
+        const dim3 grid((unsigned)(now * a.splits));
+        if (flat) {
+            distill_plan<E><<<grid, dim3(64), bytes, stream>>>(a);
+            distill_flat<E><<<dim3((unsigned)(now * a.tiles)), dim3(256), 0, stream>>>(a);
+            if (a.k)
+                distill_named<E><<<dim3((unsigned)((now * a.k + 255) / 256)), dim3(256), 0, stream>>>(a, now);
+        } else if (what == kGrad) {
+            distill_rows<E, 256, kGrad><<<grid, dim3(256), bytes, stream>>>(a);
         } else if (a.splits == 1) {
             if (what == kLoss)
-                distill_rows<E, kLoss><<<grid, block, bytes, stream>>>(a);
+                distill_rows<E, 256, kLoss><<<grid, dim3(256), bytes, stream>>>(a);
             else
-                distill_rows<E, kLoss | kGrad><<<grid, block, bytes, stream>>>(a);
+                // fewer rows at a time, so that they are still in the caches when they are read again
+                distill_rows<E, 512, kLoss | kGrad><<<grid, dim3(512), bytes, stream>>>(a);
         } else {
-            distill_stats<E><<<grid, block, 0, stream>>>(a);
+            distill_stats<E><<<grid, dim3(kStatsThreads), 0, stream>>>(a);
             if (what == kLoss)
-                distill_rows<E, kLoss | kParts><<<dim3((unsigned)now), block, bytes, stream>>>(a);
+                distill_rows<E, 64, kLoss | kParts><<<dim3((unsigned)now), dim3(64), bytes, stream>>>(a);
             else
-                distill_rows<E, kLoss | kGrad | kParts><<<grid, block, bytes, stream>>>(a);
+                distill_rows<E, 256, kLoss | kGrad | kParts><<<grid, dim3(256), bytes, stream>>>(a);
         }
         if (const int status = nbh_launch_status())
             return status;
@@ -357,10 +469,14 @@ int launch_distill(Distill a, int64_t rows, int what, hipStream_t stream)
 extern "C" size_t nbh_rows_distill_workspace(int64_t rows, int64_t vocab, int64_t k, int dtype, int what)
 {
     if (rows <= 0 || vocab < 0 || vocab > INT32_MAX || k < 0 || k > NBH_ROW_TOP_MOST || dtype < 0 ||
-        dtype > NBH_ROW_BF16 || !(what & NBH_DISTILL_LOSS))
+        dtype > NBH_ROW_BF16 || what < kLoss || what > (kLoss | kGrad))
         return 0;
-    const Split s = split_of(rows, vocab, dtype);
-    return s.splits == 1 ? 0 : (size_t)rows * (s.splits * sizeof(nbh_softmax) + (size_t)k * sizeof(float));
+    const Spread s = spread_of(rows, vocab, dtype, what);
+    if (s.flat)
+        return (size_t)rows * (sizeof(Plan) + (size_t)k * sizeof(Named));
+    return s.splits == 1 || !(what & kLoss)
+               ? 0
+               : (size_t)rows * (s.splits * sizeof(nbh_softmax) + (size_t)k * sizeof(float));
 }
 
 extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_stream_t stream)
@@ -379,13 +495,13 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     const size_t need = nbh_rows_distill_workspace(p->rows, p->vocab, p->k, (int)p->dtype, (int)p->what);
     if (need && (!p->workspace || p->workspace_bytes < (int64_t)need || ((uintptr_t)p->workspace & 15)))
         return (int)hipErrorInvalidValue;
-    const Split split = split_of(p->rows, p->vocab, (int)p->dtype);
+    const Spread spread = spread_of(p->rows, p->vocab, (int)p->dtype, (int)p->what);
     Distill a = {};
     a.student = (const char *)p->student;
     a.stride = p->stride;
     a.vocab = p->vocab;
-    a.slice = split.slice;
-    a.splits = split.splits;
+    a.slice = spread.slice;
+    a.splits = spread.splits;
     a.k = (int)p->k;
     a.index_bytes = (int)p->index_bytes;
     a.values_dtype = (int)p->values_dtype;
@@ -405,16 +521,18 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     a.grad = (char *)p->grad;
     a.grad_stride = p->grad_stride;
     a.parts = (nbh_softmax *)p->workspace;
-    a.targets = (float *)(a.parts + p->rows * split.splits);
+    a.targets = (float *)(a.parts + p->rows * spread.splits);
+    a.plans = (Plan *)p->workspace;
+    a.named = (Named *)(a.plans + p->rows);
 
     const hipStream_t s = nbh_hip_stream(stream);
     nbh_stream_report report(s);
     switch (p->dtype) {
     case NBH_ROW_F32:
-        return launch_distill<nbh_row_f32>(a, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f32>(a, spread.flat, p->rows, (int)p->what, s);
     case NBH_ROW_F16:
-        return launch_distill<nbh_row_f16>(a, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f16>(a, spread.flat, p->rows, (int)p->what, s);
     default:
-        return launch_distill<nbh_row_bf16>(a, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_bf16>(a, spread.flat, p->rows, (int)p->what, s);
     }
 }

@@ -544,7 +544,8 @@ def distill_loss(student, values, indices, *, temperature=1.0, teacher_lse=None,
     return loss, lse
 
 
-def distill_grad(grad_loss, student, values, indices, lse, *, temperature=1.0, teacher_lse=None, out=None, stream=0):
+def distill_grad(grad_loss, student, values, indices, lse, *, temperature=1.0, teacher_lse=None, out=None,
+                 workspace=None, stream=0):
     """The gradient of sum(grad_loss * loss) with respect to `student`, from the `lse` that
     distill_loss returned:
 
@@ -554,7 +555,7 @@ def distill_grad(grad_loss, student, values, indices, lse, *, temperature=1.0, t
     out       : of the student's shape and type; may be `student` itself
     A row without entries, or with grad_loss 0, has gradient 0.  Other arguments as for distill_loss.
     """
-    return _distill(_GRAD, grad_loss, student, values, indices, temperature, teacher_lse, None, lse, out, None,
+    return _distill(_GRAD, grad_loss, student, values, indices, temperature, teacher_lse, None, lse, out, workspace,
                     stream)[2]
 
 

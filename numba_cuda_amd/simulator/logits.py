@@ -255,7 +255,8 @@ def distill_loss(student, values, indices, *, temperature=1.0, teacher_lse=None,
     return _distill(True, False, None, student, values, indices, temperature, teacher_lse, loss, lse, None, stream)[:2]
 
 
-def distill_grad(grad_loss, student, values, indices, lse, *, temperature=1.0, teacher_lse=None, out=None, stream=0):
+def distill_grad(grad_loss, student, values, indices, lse, *, temperature=1.0, teacher_lse=None, out=None,
+                 workspace=None, stream=0):
     return _distill(False, True, grad_loss, student, values, indices, temperature, teacher_lse, None, lse, out,
                     stream)[2]
 

@@ -343,3 +343,16 @@ def test_no_rows(call):
         empty = logits.distill_loss_and_grad(1.0, cuda.device_array((2, 0), np.float32), cuda.to_device(
             np.zeros((2, 3), np.float32)), cuda.to_device(np.zeros((2, 3), np.int32)))
         assert not empty[0].copy_to_host().any() and (empty[1].copy_to_host() == -np.inf).all()
+
+
+@pytest.mark.parametrize("name", cases.DTYPES)
+@pytest.mark.parametrize("in_place, repeated", [(False, False), (True, True)])
+def test_large_gradient_by_itself(name, in_place, repeated):
+    rows, vocab = (700, 26003) if name == "float32" else (1300, 27001)      # over 64 MiB: three launches
+    assert logits.distill_workspace(rows, vocab, 20, cases.np_dtype(name), loss=False, grad=True) > 0
+    cases.check_distill(cuda, rows, vocab, name, 20, what="apart", in_place=in_place, repeated=repeated,
+                        pad=0 if in_place else 5, full=not repeated)
+
+
+def test_large_gradient_of_special_rows():
+    cases.check_distill(cuda, 900, 20011, "float32", 6, what="apart", kind="edge", temperature=0.7)
