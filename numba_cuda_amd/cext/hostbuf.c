@@ -12,6 +12,9 @@
  *   extents_of(shape, strides, itemsize)  the same from a description, relative to 0
  *   reduce_into(codes, arr, res, init, stream, ...)  Reduce.__call__ with `res=` for the plain
  *                           case, from the array objects to the launch (described at the function)
+ *   row_view(obj, kinds), vector_view(obj, kinds, length)  address, shape and stride of a plain
+ *                           2-d or 1-d device array or torch tensor, for the row operators
+ *                           (described at the functions)
  *   call_reduce(entry, op, dtype, in, n, stride, init, out, scratch, scratch_bytes, stream)
  *                           calls the library's nbh_reduce through its address, all
  *                           arguments plain integers: the launch path of Reduce.__call__
@@ -328,7 +331,134 @@ out:
     Py_RETURN_NOTIMPLEMENTED;
 }
 
+/* The arguments of the row operators (kernels/logits.py), a dozen of which a call of a few
+ * microseconds may have: what the Python path (_input / _output with _as_rows or _as_vector)
+ * finds out about an ordinary argument, in one call.  An ordinary argument is an instance of
+ * exactly the device array class or of a class listed in `kinds` under its type object, not of a
+ * subclass, whose dtype object is a key of `kinds`; the value is (item size, code).  Anything
+ * else - another class, a tensor that is not on the device, another number of axes, another
+ * length, items that do not lie next to each other, an address or row stride that is not a
+ * multiple of the item size - gives None, and the Python path takes the argument (and raises
+ * what there is to raise).  Torch's strides count items, a device array's bytes: `kinds[type]`
+ * is True for the former. */
+static PyObject *str_is_cuda, *str_dtype, *str_shape, *str_stride, *str_strides, *str_data_ptr, *str_gpu_data,
+    *str_device_pointer;
+
+typedef struct {
+    unsigned long long address;
+    long long shape[2], strides[2]; /* strides in bytes */
+    int ndim;
+    long long itemsize;
+    PyObject *code; /* borrowed from kinds */
+} plain_view;
+
+/* 0: found, 1: not an ordinary argument, -1: an exception is set */
+static int plain_view_of(PyObject *obj, PyObject *kinds, plain_view *v)
+{
+    PyObject *in_items = PyDict_GetItemWithError(kinds, (PyObject *)Py_TYPE(obj)); /* borrowed */
+    if (!in_items)
+        return PyErr_Occurred() ? -1 : 1;
+    const int tensor = in_items == Py_True;
+    PyObject *dtype = NULL, *shape = NULL, *strides = NULL, *address = NULL, *data = NULL;
+    int rc = -1;
+    if (tensor) {
+        PyObject *flag = PyObject_GetAttr(obj, str_is_cuda);
+        if (!flag)
+            return -1;
+        Py_DECREF(flag);
+        if (flag != Py_True)
+            return 1;
+    }
+    dtype = PyObject_GetAttr(obj, str_dtype);
+    if (!dtype)
+        goto out;
+    PyObject *kind = PyDict_GetItemWithError(kinds, dtype); /* borrowed */
+    if (!kind) {
+        rc = PyErr_Occurred() ? -1 : 1;
+        goto out;
+    }
+    shape = PyObject_GetAttr(obj, str_shape);
+    strides = !shape ? NULL : tensor ? PyObject_CallMethodNoArgs(obj, str_stride) : PyObject_GetAttr(obj, str_strides);
+    if (!strides)
+        goto out;
+    rc = 1;
+    if (!PyTuple_Check(kind) || PyTuple_GET_SIZE(kind) != 2 || !PyTuple_Check(shape) || !PyTuple_Check(strides) ||
+        PyTuple_GET_SIZE(shape) > 2 || PyTuple_GET_SIZE(shape) != PyTuple_GET_SIZE(strides))
+        goto out;
+    if (tensor) {
+        address = PyObject_CallMethodNoArgs(obj, str_data_ptr);
+    } else {
+        data = PyObject_GetAttr(obj, str_gpu_data);
+        address = data ? PyObject_GetAttr(data, str_device_pointer) : NULL;
+        if (!address) { /* memory of another kind: the Python path knows how to ask it */
+            PyErr_Clear();
+            goto out;
+        }
+    }
+    if (!address) {
+        rc = -1;
+        goto out;
+    }
+    v->address = PyLong_AsUnsignedLongLong(address);
+    v->itemsize = PyLong_AsLongLong(PyTuple_GET_ITEM(kind, 0));
+    v->code = PyTuple_GET_ITEM(kind, 1);
+    v->ndim = (int)PyTuple_GET_SIZE(shape);
+    for (int k = 0; k < v->ndim; ++k) {
+        v->shape[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k));
+        v->strides[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, k)) * (tensor ? v->itemsize : 1);
+    }
+    rc = PyErr_Occurred() ? -1 : 0;
+out:
+    Py_XDECREF(dtype);
+    Py_XDECREF(shape);
+    Py_XDECREF(strides);
+    Py_XDECREF(address);
+    Py_XDECREF(data);
+    return rc;
+}
+
+/* (address, rows, columns, bytes from row to row, code) or None */
+static PyObject *hb_row_view(PyObject *mod, PyObject *const *args, Py_ssize_t nargs)
+{
+    plain_view v;
+    if (nargs != 2 || !PyDict_CheckExact(args[1])) {
+        PyErr_SetString(PyExc_TypeError, "row_view(obj, kinds)");
+        return NULL;
+    }
+    const int rc = plain_view_of(args[0], args[1], &v);
+    if (rc < 0)
+        return NULL;
+    if (rc || v.ndim != 2 || (v.shape[1] > 1 && v.strides[1] != v.itemsize) || v.address % v.itemsize ||
+        (v.shape[0] > 1 && v.strides[0] % v.itemsize))
+        Py_RETURN_NONE;
+    return Py_BuildValue("KLLLO", v.address, v.shape[0], v.shape[1], v.shape[0] > 1 ? v.strides[0] : 0LL, v.code);
+}
+
+/* (address, items, item size) or None; a negative length takes any */
+static PyObject *hb_vector_view(PyObject *mod, PyObject *const *args, Py_ssize_t nargs)
+{
+    plain_view v;
+    if (nargs != 3 || !PyDict_CheckExact(args[1])) {
+        PyErr_SetString(PyExc_TypeError, "vector_view(obj, kinds, length)");
+        return NULL;
+    }
+    const long long length = PyLong_AsLongLong(args[2]);
+    if (length == -1 && PyErr_Occurred())
+        return NULL;
+    const int rc = plain_view_of(args[0], args[1], &v);
+    if (rc < 0)
+        return NULL;
+    if (rc || v.ndim != 1 || (length >= 0 && v.shape[0] != length) ||
+        (v.shape[0] > 1 && v.strides[0] != v.itemsize) || v.address % v.itemsize)
+        Py_RETURN_NONE;
+    return Py_BuildValue("KLL", v.address, v.shape[0], v.itemsize);
+}
+
 static PyMethodDef hb_methods[] = {
+    {"row_view", (PyCFunction)(void (*)(void))hb_row_view, METH_FASTCALL,
+     "row_view(obj, kinds) -> (address, rows, columns, stride, code) | None"},
+    {"vector_view", (PyCFunction)(void (*)(void))hb_vector_view, METH_FASTCALL,
+     "vector_view(obj, kinds, length) -> (address, items, item size) | None"},
     {"reduce_into", (PyCFunction)(void (*)(void))hb_reduce_into, METH_FASTCALL,
      "reduce_into(codes, arr, res, init, stream, thread_state, stream_type, init_cache, lib) -> None | status | NotImplemented"},
     {"call_reduce", (PyCFunction)(void (*)(void))hb_call_reduce, METH_FASTCALL,
@@ -356,7 +486,16 @@ PyMODINIT_FUNC PyInit__hostbuf(void)
     str_prepared = PyUnicode_InternFromString("prepared");
     str_scratch = PyUnicode_InternFromString("_scratch");
     str_entry = PyUnicode_InternFromString("_reduce_entry");
-    if (!str_rk || !str_handle || !str_ctx || !str_prepared || !str_scratch || !str_entry) {
+    str_is_cuda = PyUnicode_InternFromString("is_cuda");
+    str_dtype = PyUnicode_InternFromString("dtype");
+    str_shape = PyUnicode_InternFromString("shape");
+    str_stride = PyUnicode_InternFromString("stride");
+    str_strides = PyUnicode_InternFromString("strides");
+    str_data_ptr = PyUnicode_InternFromString("data_ptr");
+    str_gpu_data = PyUnicode_InternFromString("gpu_data");
+    str_device_pointer = PyUnicode_InternFromString("device_pointer");
+    if (!str_is_cuda || !str_dtype || !str_shape || !str_stride || !str_strides || !str_data_ptr || !str_gpu_data ||
+        !str_device_pointer || !str_rk || !str_handle || !str_ctx || !str_prepared || !str_scratch || !str_entry) {
         Py_DECREF(m);
         return NULL;
     }

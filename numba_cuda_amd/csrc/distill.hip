@@ -7,15 +7,15 @@
 // One workgroup per row: its first wavefront brings the teacher's entries to LDS while the others begin
 // the pass over the row that gives its maximum and sum together; a second pass, backwards, so that it finds
 // the end of the first in the caches, writes the gradient as a * 2^((s - m) * c) for every entry, and behind
-// a barrier the few entries the teacher names are written again with their p_j taken off.  Few rows are
-// split over workgroups: a launch for the statistics of the stretches, then one that joins them and works
-// on the stretches.  A large gradient by itself is a copy with arithmetic: a launch prepares two numbers
+// a barrier the few entries the teacher names are written again with their p_j taken off.  The loss
+// alone, and few rows, are spread: small workgroups in the order of memory for the statistics, then a launch
+// that joins them and does the rest.  A large gradient by itself is a copy with arithmetic: a launch prepares two numbers
 // for each row, small workgroups in memory order do the copy, a last launch writes the named entries.
 #include "rows.h"
 
 namespace {
 
-constexpr int kStatsThreads = 256;
+constexpr int kStatsThreads = 64, kStatsVecs = 8;      // 8 KiB per workgroup
 constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f;       // log2(e) and its rounding
 constexpr float kLn2 = 0.693147180559945309f;
 
@@ -47,28 +47,54 @@ struct Distill {
     float *targets;                      // per row: the student's values at the teacher's k indices
     Plan *plans;                         // per row
     Named *named;                        // per row and teacher's entry
-    int tiles;
+    int tiles;                           // workgroups per row of distill_stats or distill_flat
 };
 
+// The statistics of 8 KiB of a row per workgroup, in the order of memory, one pair of numbers per wavefront.
 template <typename E>
 __global__ __launch_bounds__(kStatsThreads) void distill_stats(Distill a)
 {
-    constexpr int T = kStatsThreads;
-    __shared__ nbh_softmax room[T / 64];
-    const int64_t row = a.row0 + blockIdx.x / a.splits;
-    const int split = blockIdx.x % a.splits;
+    constexpr int T = kStatsThreads, kItems = E::items;
+    const int64_t at = blockIdx.x / a.tiles, row = a.row0 + at;
+    const int tile = blockIdx.x % a.tiles;
     const typename E::item *in = reinterpret_cast<const typename E::item *>(a.student + row * a.stride);
-    const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
-    const nbh_softmax stats = nbh_softmax_group<T>(nbh_row_stats<E, T, false>(in, begin, end, a.scale), a.scale, room);
-    if (threadIdx.x == 0)
-        a.parts[(row - a.row0) * a.splits + split] = stats;
+    const int64_t first = (int64_t)tile * T * kStatsVecs * kItems - nbh_row_before<E>(in);
+    nbh_u32x4 raw[kStatsVecs];
+    if (first >= 0 && first + T * kStatsVecs * kItems <= a.vocab) {
+#pragma unroll
+        for (int j = 0; j < kStatsVecs; ++j)
+            raw[j] = E::template load<true>(in + first + (j * T + threadIdx.x) * kItems);
+    } else {
+#pragma unroll
+        for (int j = 0; j < kStatsVecs; ++j)
+            raw[j] = nbh_row_load_raw<E, true>(in, first + (j * T + (int)threadIdx.x) * kItems, a.vocab, E::lowest);
+    }
+    nbh_softmax stats = nbh_softmax_empty();
+#pragma unroll
+    for (int j = 0; j < kStatsVecs; ++j) {
+        float f[kItems];
+        E::unpack(raw[j], f);
+        nbh_softmax_add(stats, f, nbh_row_most(f), a.scale);
+    }
+    stats = nbh_softmax_wave(stats, a.scale);
+    if ((threadIdx.x & 63) == 0)
+        a.parts[(at * a.tiles + tile) * (T / 64) + threadIdx.x / 64] = stats;
     // The loss needs these of the whole row, and the gradient may be written over the row while another
     // stretch's workgroup still works on the loss: they are set aside.
-    if (split == 0)
+    if (a.targets && tile == 0)
         for (int j = threadIdx.x; j < a.k; j += T) {
-            const int64_t at = nbh_row_int(a.indices + row * a.indices_stride, a.index_bytes, j);
-            a.targets[(row - a.row0) * a.k + j] = at >= 0 && at < a.vocab ? E::get(in[at]) : 0.0f;
+            const int64_t index = nbh_row_int(a.indices + row * a.indices_stride, a.index_bytes, j);
+            a.targets[at * a.k + j] = index >= 0 && index < a.vocab ? E::get(in[index]) : 0.0f;
         }
+}
+// What they add up to; every wavefront for itself.
+__device__ __forceinline__ nbh_softmax joined_stats(const Distill &a, int64_t at)
+{
+    const int parts = a.tiles * (kStatsThreads / 64);
+    nbh_softmax stats = nbh_softmax_empty();
+    for (int i = threadIdx.x & 63; i < parts; i += 64)
+        stats = nbh_softmax_join(stats, a.parts[at * parts + i], a.scale);
+    return nbh_softmax_wave(stats, a.scale);
 }
 
 __device__ __forceinline__ float wave_add(float x)
@@ -146,9 +172,9 @@ __device__ void load_teacher(const Distill &a, int64_t row, int64_t begin, int64
         t.index[j] = present ? (int32_t)at : -1;
         t.log_p[j] = value;
         if (present) {
-            t.student[j] = WHAT & kParts                ? a.targets[(row - a.row0) * a.k + j]
-                           : at >= begin && at < end ? E::get(in[at])
-                                                        : 0.0f;
+            t.student[j] = (WHAT & (kParts | kGrad)) == (kParts | kGrad) ? a.targets[(row - a.row0) * a.k + j]
+                           : at >= begin && at < end                     ? E::get(in[at])
+                                                                         : 0.0f;
             peak = fmaxf(peak, fminf(value, FLT_MAX));
             some = 1;
         }
@@ -292,9 +318,7 @@ template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void dist
     if (WHAT & kLoss) {
         nbh_softmax stats;
         if (WHAT & kParts) {
-            stats = a.parts[(row - a.row0) * a.splits];
-            for (int s = 1; s < a.splits; ++s)
-                stats = nbh_softmax_join(stats, a.parts[(row - a.row0) * a.splits + s], a.scale);
+            stats = joined_stats(a, row - a.row0);
             __syncthreads();
         } else {
             stats = nbh_softmax_group<T>(nbh_row_stats<E, T, false>(in, 0, a.vocab, a.scale), a.scale, room);
@@ -368,32 +392,49 @@ template <typename E> __global__ __launch_bounds__(64) void distill_plan(Distill
     for (int j = threadIdx.x; j < a.k; j += 64)
         a.named[(row - a.row0) * a.k + j] = zero ? Named{-1, 0.0f} : named_of(a, teacher, j, student, whole, factor);
 }
-// Second: 4 KiB of a row per workgroup, in the order of memory.
-template <typename E> __global__ __launch_bounds__(256) void distill_flat(Distill a)
+// Second: small workgroups in the order of memory.
+constexpr int kFlatThreads = 64, kFlatVecs = 1;
+template <typename E> __global__ __launch_bounds__(kFlatThreads) void distill_flat(Distill a)
 {
     typedef typename E::item item;
-    constexpr int kItems = E::items;
+    constexpr int kItems = E::items, T = kFlatThreads, V = kFlatVecs;
     const int64_t row = blockIdx.x / a.tiles;
-    const int64_t at = ((int64_t)(blockIdx.x % a.tiles) * 256 + threadIdx.x) * kItems;
-    if (at >= a.vocab)
-        return;
     const item *in = reinterpret_cast<const item *>(a.student + (a.row0 + row) * a.stride);
     item *out = reinterpret_cast<item *>(a.grad + (a.row0 + row) * a.grad_stride);
-    float f[kItems];
-    nbh_row_load<E, true>(in, at, a.vocab, 0.0f, f);
+    const int64_t first = (int64_t)(blockIdx.x % a.tiles) * T * V * kItems - nbh_row_before<E>(in);
     const Plan plan = a.plans[row];
-    const float product = plan.peak * a.scale;
-    if (plan.zero) {
-        for (int i = 0; i < kItems; ++i)
-            f[i] = 0.0f;
-    } else if (nbh_softmax_near(product)) {
-        for (int i = 0; i < kItems; ++i)
-            f[i] = plan.whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+    nbh_u32x4 raw[V];
+    const bool full = first >= 0 && first + T * V * kItems <= a.vocab;
+    if (full) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            raw[j] = E::template load<true>(in + first + (j * T + threadIdx.x) * kItems);
     } else {
-        for (int i = 0; i < kItems; ++i)
-            f[i] = plan.whole * nbh_exp2((f[i] - plan.peak) * a.scale);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            raw[j] = nbh_row_load_raw<E, true>(in, first + (j * T + (int)threadIdx.x) * kItems, a.vocab, 0);
     }
-    nbh_row_store<E, true>(out, at, a.vocab, f);
+    const float product = plan.peak * a.scale;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        float f[kItems];
+        E::unpack(raw[j], f);
+        if (plan.zero) {
+            for (int i = 0; i < kItems; ++i)
+                f[i] = 0.0f;
+        } else if (nbh_softmax_near(product)) {
+            for (int i = 0; i < kItems; ++i)
+                f[i] = plan.whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+        } else {
+            for (int i = 0; i < kItems; ++i)
+                f[i] = plan.whole * nbh_exp2((f[i] - plan.peak) * a.scale);
+        }
+        const int64_t at = first + (j * T + (int)threadIdx.x) * kItems;
+        if (full)
+            nbh_store16<sizeof(item), true>(out + at, E::pack(f));
+        else
+            nbh_row_store<E, true>(out, at, a.vocab, f);
+    }
 }
 // Third: a lane per entry the teacher names.
 template <typename E> __global__ __launch_bounds__(256) void distill_named(Distill a, int64_t rows)
@@ -407,56 +448,63 @@ template <typename E> __global__ __launch_bounds__(256) void distill_named(Disti
 }
 
 // How a call is spread.
-//   splits, slice   stretches of a row: one workgroup per row from 1024 rows on, else workgroups for four per
-//                   compute unit
-//   flat            the gradient by itself in three launches, where its rows hold 64 MiB or more
+//   kRows    one workgroup per row does everything
+//   kParts   launches of small workgroups for the statistics, then a wavefront per row for the loss alone, or
+//            with the gradient `splits` workgroups per row, four per compute unit, for stretches of `slice`
+//   kFlat    the gradient by itself in three launches, where the rows hold 64 MiB or more
+enum Way { kRows, kInParts, kFlat };
 struct Spread {
-    bool flat;
-    int splits;
+    Way way;
+    int tiles, splits;
     int64_t slice;
 };
-Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what)
+// `spare`: entries before a row's beginning that its first vector may hold
+Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what, int spare)
 {
     const int64_t items = dtype == NBH_ROW_F32 ? 4 : 8;
-    if (what == kGrad && rows * vocab >= ((int64_t)64 << 20) / 16 * items)
-        return {true, 1, vocab};
-    const int64_t chunk = kStatsThreads * kNbhAhead * items;
+    const int64_t chunk = kStatsThreads * kNbhAhead * items, tile = kStatsThreads * kStatsVecs * items;
+    const int64_t flat = kFlatThreads * kFlatVecs * items;
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
+    if (what == kGrad && rows * vocab >= ((int64_t)64 << 20) / 16 * items)
+        return {kFlat,
+                (int)((vocab + spare + flat - 1) / flat), 1, vocab};
+    const int tiles = (int)((vocab + spare + tile - 1) / tile);
+    if (what == kLoss)
+        return {chunks > 1 ? kInParts : kRows, tiles, 1, vocab};
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
         splits = chunks;
     const int64_t each = (chunks + splits - 1) / splits;
-    return {false, (int)((chunks + each - 1) / each), each * chunk};
+    splits = (chunks + each - 1) / each;
+    return {what != kGrad && splits > 1 ? kInParts : kRows, tiles, (int)splits, each * chunk};
 }
 
 template <typename E>
-int launch_distill(Distill a, bool flat, int64_t rows, int what, hipStream_t stream)
+int launch_distill(Distill a, Way way, int64_t rows, int what, hipStream_t stream)
 {
     const size_t bytes = Teacher::bytes(a.k);
-    a.tiles = (int)((a.vocab + 256 * E::items - 1) / (256 * E::items));
-    const int64_t most = NBH_ROW_MOST_GROUPS / (flat ? a.tiles : a.splits);
+    const int64_t most = NBH_ROW_MOST_GROUPS / (way == kRows ? a.splits : a.tiles);
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
-        const dim3 grid((unsigned)(now * a.splits));
-        if (flat) {
-            distill_plan<E><<<grid, dim3(64), bytes, stream>>>(a);
-            distill_flat<E><<<dim3((unsigned)(now * a.tiles)), dim3(256), 0, stream>>>(a);
+        const dim3 each((unsigned)now), split((unsigned)(now * a.splits)), tiled((unsigned)(now * a.tiles));
+        if (way == kFlat) {
+            distill_plan<E><<<each, dim3(64), bytes, stream>>>(a);
+            distill_flat<E><<<tiled, dim3(kFlatThreads), 0, stream>>>(a);
             if (a.k)
                 distill_named<E><<<dim3((unsigned)((now * a.k + 255) / 256)), dim3(256), 0, stream>>>(a, now);
+        } else if (way == kInParts) {
+            distill_stats<E><<<tiled, dim3(kStatsThreads), 0, stream>>>(a);
+            if (what == kLoss)
+                distill_rows<E, 64, kLoss | kParts><<<each, dim3(64), bytes, stream>>>(a);
+            else
+                distill_rows<E, 256, kLoss | kGrad | kParts><<<split, dim3(256), bytes, stream>>>(a);
         } else if (what == kGrad) {
-            distill_rows<E, 256, kGrad><<<grid, dim3(256), bytes, stream>>>(a);
-        } else if (a.splits == 1) {
-            if (what == kLoss)
-                distill_rows<E, 256, kLoss><<<grid, dim3(256), bytes, stream>>>(a);
-            else
-                // fewer rows at a time, so that they are still in the caches when they are read again
-                distill_rows<E, 512, kLoss | kGrad><<<grid, dim3(512), bytes, stream>>>(a);
+            distill_rows<E, 256, kGrad><<<split, dim3(256), bytes, stream>>>(a);
+        } else if (what == kLoss) {
+            distill_rows<E, 256, kLoss><<<each, dim3(256), bytes, stream>>>(a);
         } else {
-            distill_stats<E><<<grid, dim3(kStatsThreads), 0, stream>>>(a);
-            if (what == kLoss)
-                distill_rows<E, 64, kLoss | kParts><<<dim3((unsigned)now), dim3(64), bytes, stream>>>(a);
-            else
-                distill_rows<E, 256, kLoss | kGrad | kParts><<<grid, dim3(256), bytes, stream>>>(a);
+            // fewer rows at a time, so that they are still in the caches when they are read again
+            distill_rows<E, 512, kLoss | kGrad><<<each, dim3(512), bytes, stream>>>(a);
         }
         if (const int status = nbh_launch_status())
             return status;
@@ -471,12 +519,13 @@ extern "C" size_t nbh_rows_distill_workspace(int64_t rows, int64_t vocab, int64_
     if (rows <= 0 || vocab < 0 || vocab > INT32_MAX || k < 0 || k > NBH_ROW_TOP_MOST || dtype < 0 ||
         dtype > NBH_ROW_BF16 || what < kLoss || what > (kLoss | kGrad))
         return 0;
-    const Spread s = spread_of(rows, vocab, dtype, what);
-    if (s.flat)
+    const Spread s = spread_of(rows, vocab, dtype, what, 7);
+    if (s.way == kFlat)
         return (size_t)rows * (sizeof(Plan) + (size_t)k * sizeof(Named));
-    return s.splits == 1 || !(what & kLoss)
-               ? 0
-               : (size_t)rows * (s.splits * sizeof(nbh_softmax) + (size_t)k * sizeof(float));
+    if (s.way == kInParts)
+        return (size_t)rows * ((size_t)s.tiles * (kStatsThreads / 64) * sizeof(nbh_softmax) +
+                               (what & kGrad ? (size_t)k * sizeof(float) : 0));
+    return 0;
 }
 
 extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_stream_t stream)
@@ -495,7 +544,8 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     const size_t need = nbh_rows_distill_workspace(p->rows, p->vocab, p->k, (int)p->dtype, (int)p->what);
     if (need && (!p->workspace || p->workspace_bytes < (int64_t)need || ((uintptr_t)p->workspace & 15)))
         return (int)hipErrorInvalidValue;
-    const Spread spread = spread_of(p->rows, p->vocab, (int)p->dtype, (int)p->what);
+    const Spread spread = spread_of(p->rows, p->vocab, (int)p->dtype, (int)p->what,
+                                    nbh_row_spare(p->student, p->stride, (int)p->dtype));
     Distill a = {};
     a.student = (const char *)p->student;
     a.stride = p->stride;
@@ -521,7 +571,9 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     a.grad = (char *)p->grad;
     a.grad_stride = p->grad_stride;
     a.parts = (nbh_softmax *)p->workspace;
-    a.targets = (float *)(a.parts + p->rows * spread.splits);
+    a.tiles = spread.tiles;
+    if (grad)
+        a.targets = (float *)(a.parts + p->rows * spread.tiles * (kStatsThreads / 64));
     a.plans = (Plan *)p->workspace;
     a.named = (Named *)(a.plans + p->rows);
 
@@ -529,10 +581,10 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     nbh_stream_report report(s);
     switch (p->dtype) {
     case NBH_ROW_F32:
-        return launch_distill<nbh_row_f32>(a, spread.flat, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f32>(a, spread.way, p->rows, (int)p->what, s);
     case NBH_ROW_F16:
-        return launch_distill<nbh_row_f16>(a, spread.flat, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f16>(a, spread.way, p->rows, (int)p->what, s);
     default:
-        return launch_distill<nbh_row_bf16>(a, spread.flat, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_bf16>(a, spread.way, p->rows, (int)p->what, s);
     }
 }

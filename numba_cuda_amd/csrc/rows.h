@@ -117,16 +117,27 @@ template <typename E> struct nbh_row_half {
     }
 };
 
-// The 16 bytes at element `at` of a row of `n` elements; elements behind the row's end read as `fill`, the
-// raw one as its bits.
+// Elements from the last multiple of 16 bytes before a row to its beginning.  Vectors counted from there are
+// aligned: a wavefront's load then covers 8 cache lines, not 9 (10 % of a row's reading time).
+template <typename E> __device__ __forceinline__ int nbh_row_before(const typename E::item *row)
+{
+    return (int)((uintptr_t)row / sizeof(typename E::item) % E::items);
+}
+// The most that can be for the rows of an array.
+static inline int nbh_row_spare(const void *address, int64_t stride, int dtype)
+{
+    return ((uintptr_t)address | (uintptr_t)stride) & 15 ? (dtype == NBH_ROW_F32 ? 3 : 7) : 0;
+}
+// The 16 bytes at element `at` of a row of `n` elements; elements before the row and behind its end read as
+// `fill`, the raw one as its bits.
 template <typename E, bool NT>
 __device__ __forceinline__ nbh_u32x4 nbh_row_load_raw(const typename E::item *row, int64_t at, int64_t n, uint32_t fill)
 {
-    if (at + E::items <= n)
+    if (at >= 0 && at + E::items <= n)
         return E::template load<NT>(row + at);
     nbh_u32x4 v = {};
     for (int i = 0; i < E::items; ++i) {
-        const uint32_t bits = at + i < n ? E::bits(row[at + i]) : fill;
+        const uint32_t bits = at + i >= 0 && at + i < n ? E::bits(row[at + i]) : fill;
         if (sizeof(typename E::item) == 4)
             v[i] = bits;
         else
@@ -138,21 +149,21 @@ template <typename E, bool NT>
 __device__ __forceinline__ void nbh_row_load(const typename E::item *row, int64_t at, int64_t n, float fill,
                                              float (&f)[E::items])
 {
-    if (at + E::items <= n) {
+    if (at >= 0 && at + E::items <= n) {
         E::unpack(nbh_load16<sizeof(typename E::item), NT>(row + at), f);
     } else {
         for (int i = 0; i < E::items; ++i)
-            f[i] = at + i < n ? E::get(row[at + i]) : fill;
+            f[i] = at + i >= 0 && at + i < n ? E::get(row[at + i]) : fill;
     }
 }
 template <typename E, bool NT>
 __device__ __forceinline__ void nbh_row_store(typename E::item *row, int64_t at, int64_t n, const float (&f)[E::items])
 {
-    if (at + E::items <= n) {
+    if (at >= 0 && at + E::items <= n) {
         nbh_store16<sizeof(typename E::item), NT>(row + at, E::pack(f));
     } else {
         for (int i = 0; i < E::items; ++i)
-            if (at + i < n)
+            if (at + i >= 0 && at + i < n)
                 row[at + i] = E::put(f[i]);
     }
 }
@@ -227,14 +238,20 @@ __device__ __forceinline__ float nbh_softmax_lse(nbh_softmax s, float temperatur
     return nbh_softmax_near(product) ? (product + log2f(s.sum)) * 0.693147180559945309f
                                      : s.peak / temperature + logf(s.sum);
 }
-// Over a workgroup of `T` lanes; `room` holds T / 64 entries.  Every lane gets the result.
-template <int T>
-__device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float scale, nbh_softmax *room)
+// Over a wavefront; every lane gets the result.
+__device__ __forceinline__ nbh_softmax nbh_softmax_wave(nbh_softmax s, float scale)
 {
     for (int step = 32; step; step >>= 1) {
         const nbh_softmax other = {__shfl_xor(s.peak, step), __shfl_xor(s.sum, step)};
         s = nbh_softmax_join(s, other, scale);
     }
+    return s;
+}
+// Over a workgroup of `T` lanes; `room` holds T / 64 entries.  Every lane gets the result.
+template <int T>
+__device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float scale, nbh_softmax *room)
+{
+    s = nbh_softmax_wave(s, scale);
     if ((threadIdx.x & 63) == 0)
         room[threadIdx.x >> 6] = s;
     __syncthreads();

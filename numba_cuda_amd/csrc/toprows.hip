@@ -9,19 +9,18 @@
 //   * The groups whose maximum reaches it, about k, are listed in LDS and read again, a vector per lane;
 //     what reaches it there is appended to another list, whose order does not matter, and that is sorted:
 //     short ones by counting how many entries exceed each, others by a bitonic network.
-//   * Where too many entries reach it (masses of equal ones, rows sorted by blocks) the bound is raised by
-//     bisection over all entries, and if it ends on a value that too many share, over their indices.
-// Many rows: one workgroup does all of that for a row.  Few rows: a first launch spreads the groups'
-// maxima and the statistics of the log-sum-exp over the device, a second one does the rest.
+//   * Where too many entries reach it (masses of equal ones, rows sorted by blocks) the bound is raised, once:
+//     by bisection over all entries, and if it ends on a value that too many share, to the first of them.
+// Short rows: one workgroup does all of that for a row.  Long ones: a first launch of small workgroups in the
+// order of memory finds the groups' maxima and the statistics of the log-sum-exp, a second one does the rest.
 #include "rows.h"
 
 namespace {
 
 constexpr int kAhead = kNbhAhead;
 constexpr int kSlots = 8;                // groups per lane that the one-launch kernel remembers
-constexpr int kMaximaThreads = 256;      // first launch of two
+constexpr int kPieceVecs = 8;            // first launch of two: a wavefront takes 8 KiB at a time
 constexpr int kMostGroups = 16384;       // groups per row of the two-launch path
-constexpr int kFinishThreads = 512;
 
 struct Top {
     const char *in;
@@ -33,10 +32,9 @@ struct Top {
     int64_t indices_stride;
     float *lse;
     float temperature, scale;
-    int splits, parts;                   // two launches: workgroups per row, groups per lane of theirs
-    int64_t slice;                       // entries per workgroup
-    uint32_t *maxima;                    // [row][split][part][lane], as keys, 0 for an empty group
-    nbh_softmax *part_stats;             // [row][split]
+    int tiles, pieces;                   // two launches: workgroups per row, pieces of 8 KiB for each
+    uint32_t *maxima;                    // [row][tile][lane], as keys, 0 for an empty group
+    nbh_softmax *part_stats;             // [row][tile]
 };
 
 // Orders like the value; NaN above all, -0 as +0.  No value has key 0.
@@ -134,7 +132,7 @@ template <typename E, int T, int CAP>
 __device__ __forceinline__ void append(const typename E::item *in, int64_t at, int64_t end, uint64_t bound,
                                        uint64_t *list, Shared<T> &sh)
 {
-    if (at >= end)
+    if (at >= end || at + E::items <= 0)
         return;
     float f[E::items];
     nbh_row_load<E, false>(in, at, end, -INFINITY, f);
@@ -142,7 +140,7 @@ __device__ __forceinline__ void append(const typename E::item *in, int64_t at, i
         return;
     for (int i = 0; i < E::items; ++i) {
         const uint64_t entry = entry_of(f[i], at + i);
-        if (entry >= bound && at + i < end) {
+        if (entry >= bound && at + i >= 0 && at + i < end) {
             const int place = atomicAdd(&sh.count, 1);
             if (place < CAP)
                 list[place] = entry;
@@ -150,47 +148,116 @@ __device__ __forceinline__ void append(const typename E::item *in, int64_t at, i
     }
 }
 
-// More than CAP of the row's n entries reach the key `low`, none exceeds the key `high`: a bound that at
-// least k and at most CAP entries reach.
+// Too many of the row's n entries reach the key `low`, none exceeds the key `high`: a bound that at least k
+// and at most CAP entries reach.
 template <typename E, int T, int CAP>
 __device__ uint64_t raised_bound(const typename E::item *in, int64_t n, uint32_t low, uint32_t high, int k,
                                  Shared<T> &sh, int &turn)
 {
-    auto count = [&](auto reaches) {
-        int mine = 0;
-        for (int64_t at = (int64_t)threadIdx.x * E::items; at < n; at += T * E::items) {
-            float f[E::items];
-            nbh_row_load<E, false>(in, at, n, -INFINITY, f);
-            for (int i = 0; i < E::items; ++i)
-                mine += at + i < n && reaches(f[i], at + i);
-        }
+    constexpr int kItems = E::items;
+    auto sum = [&](int mine) {
         for (int step = 32; step; step >>= 1)
             mine += __shfl_xor(mine, step);
         return group_sum(mine, sh, turn);
     };
-    int reach = CAP + 1;
-    while (low < high && reach > CAP) {
-        const uint32_t mid = high - (high - low) / 2;
-        const int now = count([&](float x, int64_t) { return key_of(x) >= mid; });
-        if (now >= k) {
-            low = mid;
-            reach = now;
-        } else {
-            high = mid - 1;
+    auto count = [&](uint32_t key) {     // of all entries, those that reach it
+        int mine = 0;
+        for (int64_t at = (int64_t)threadIdx.x * kItems; at < n; at += T * kItems) {
+            float f[kItems];
+            nbh_row_load<E, false>(in, at, n, -INFINITY, f);
+            for (int i = 0; i < kItems; ++i)
+                mine += at + i < n && key_of(f[i]) >= key;
+        }
+        return sum(mine);
+    };
+    // The value: by bisection, unless `low` is the k-th largest already, as where all but a few entries
+    // are masked.
+    int above = low < high ? count(low + 1) : 0;             // entries that exceed `high` in what follows
+    if (above >= k) {
+        above = 0;
+        while (low < high) {
+            const uint32_t mid = high - (high - low) / 2;
+            const int now = count(mid);
+            if (now >= k && now <= CAP)
+                return (uint64_t)mid << 32;
+            if (now >= k) {
+                low = mid;
+            } else {
+                high = mid - 1;
+                above = now;
+            }
         }
     }
-    uint64_t from = (uint64_t)low << 32, to = from | 0xffffffffu;
-    while (from < to && reach > CAP) {   // low is the k-th largest value, and too many share it
-        const uint64_t mid = to - (to - from) / 2;
-        const int now = count([&](float x, int64_t index) { return entry_of(x, index) >= mid; });
-        if (now >= k) {
-            from = mid;
-            reach = now;
-        } else {
-            to = mid - 1;
+    // `above` < k entries exceed `low` and too many equal it: those with the lowest indices, in the order of
+    // memory.
+    int need = k - above;
+    for (int64_t first = 0; first < n; first += T * kItems) {
+        const int64_t at = first + threadIdx.x * kItems;
+        uint32_t equal = 0;              // bit i: entry at + i
+        if (at < n) {
+            float f[kItems];
+            nbh_row_load<E, false>(in, at, n, -INFINITY, f);
+            for (int i = 0; i < kItems; ++i)
+                equal |= at + i < n && key_of(f[i]) == low ? 1u << i : 0u;
         }
+        const int here = sum(__popc(equal));
+        if (here < need) {
+            need -= here;
+            continue;
+        }
+        int from = 0, to = T * kItems - 1;                   // the entry that makes them enough
+        while (from < to) {
+            const int mid = from + (to - from) / 2, mine = mid - (int)threadIdx.x * kItems;
+            const uint32_t upto = mine < 0 ? 0u : mine >= kItems ? ~0u : (2u << mine) - 1;
+            if (sum(__popc(equal & upto)) >= need)
+                to = mid;
+            else
+                from = mid + 1;
+        }
+        return (uint64_t)low << 32 | (uint32_t)~(uint32_t)(first + from);
     }
-    return from;
+    return (uint64_t)low << 32;          // not reached: the row holds k entries
+}
+
+// Brings at least k and at most CAP entries that reach a bound into the list, sh.count of them: first those
+// that reach `bound`; if they turn out to be too many, those that reach a raised one, which are not.
+// `most(g)`: key of the maximum of group g, 0 for an empty one; `place(g, v)`: first entry of its vector v.
+template <typename E, int T, int CAP, typename Most, typename Place>
+__device__ void collect(const typename E::item *in, int64_t n, uint64_t bound, uint32_t top, int k, uint64_t *list,
+                        int *again, Shared<T> &sh, int &turn, int groups, int vectors, Most most, Place place)
+{
+    for (int attempt = 0; attempt < 2; ++attempt) {
+        for (int g = threadIdx.x; g < groups; g += T) {
+            const uint32_t key = most(g);
+            if (key && key >= (uint32_t)(bound >> 32)) {
+                const int at = atomicAdd(&sh.groups, 1);
+                if (at < CAP)
+                    again[at] = g;
+            }
+        }
+        __syncthreads();
+        const int listed = sh.groups;
+        if (listed <= CAP) {
+            for (int64_t i = threadIdx.x; i < (int64_t)listed * vectors; i += T)
+                append<E, T, CAP>(in, place(again[i / vectors], (int)(i % vectors)), n, bound, list, sh);
+        } else if (attempt) {
+            // many groups share the raised bound's value, but few of their entries its indices
+            for (int g = threadIdx.x; g < groups; g += T) {
+                const uint32_t key = most(g);
+                if (key && key >= (uint32_t)(bound >> 32))
+                    for (int v = 0; v < vectors; ++v)
+                        append<E, T, CAP>(in, place(g, v), n, bound, list, sh);
+            }
+        }
+        __syncthreads();
+        if (attempt || (listed <= CAP && sh.count <= CAP))
+            return;
+        bound = raised_bound<E, T, CAP>(in, n, (uint32_t)(bound >> 32), top, k, sh, turn);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            sh.groups = sh.count = 0;
+        __syncthreads();
+    }
 }
 
 // Writes the k best of the list (at least k entries) in order.  The list has been written before a
@@ -313,32 +380,13 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
     }
 
     // -- what reaches it
-    uint64_t bound = (uint64_t)key << 32;
-    for (;;) {
-        const int64_t group = (int64_t)kChunk << shift;
-        for (int g = threadIdx.x; (g / T) * group < n; g += T)
-            if (maxima[g] >= (uint32_t)(bound >> 32)) {
-                const int place = atomicAdd(&sh.groups, 1);
-                if (place < CAP)
-                    again[place] = g;
-            }
-        __syncthreads();
-        if (sh.groups <= CAP) {
-            const int vectors = kAhead << shift;     // of a group
-            for (int i = threadIdx.x; i < sh.groups * vectors; i += T) {
-                const int g = again[i / vectors], v = i % vectors;
-                append<E, T, CAP>(in, (g / T) * group + (v * T + g % T) * (int64_t)kItems, n, bound, list, sh);
-            }
-            __syncthreads();
-            if (sh.count <= CAP)
-                break;
-        }
-        bound = raised_bound<E, T, CAP>(in, n, (uint32_t)(bound >> 32), top, a.k, sh, turn);
-        __syncthreads();
-        if (threadIdx.x == 0)
-            sh.groups = sh.count = 0;
-        __syncthreads();
-    }
+    const uint64_t bound = (uint64_t)key << 32;
+    const int64_t group = (int64_t)kChunk << shift;
+    const int vectors = kAhead << shift;         // of a group
+    collect<E, T, CAP>(
+        in, n, bound, top, a.k, list, again, sh, turn, (int)((n + group - 1) / group) * T, vectors,
+        [&](int g) { return maxima[g]; },
+        [&](int g, int v) { return (g / T) * group + (v * T + g % T) * (int64_t)kItems; });
     if (LSE) {
         stats = nbh_softmax_group<T>(stats, a.scale, sh.stats);
         if (threadIdx.x == 0)
@@ -347,61 +395,77 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
     write_ranked<E, T>(a, row, list, sh.count);
 }
 
-// First launch of two: the maxima of the lanes (or of the four vectors of their chunks) of a stretch.
-template <typename E, bool LSE> __global__ __launch_bounds__(kMaximaThreads) void top_maxima(Top a)
+// The largest of each eight lanes, in all eight.
+__device__ __forceinline__ uint32_t most_of_eight(uint32_t key)
 {
-    constexpr int T = kMaximaThreads, kItems = E::items;
-    __shared__ nbh_softmax room[T / 64];
-    const int64_t at = blockIdx.x / a.splits, row = a.row0 + at;
-    const int split = blockIdx.x % a.splits;
+    uint32_t other = __builtin_amdgcn_mov_dpp(key, 0xb1, 0xf, 0xf, true);        // quad_perm 1, 0, 3, 2
+    key = other > key ? other : key;
+    other = __builtin_amdgcn_mov_dpp(key, 0x4e, 0xf, 0xf, true);                 // quad_perm 2, 3, 0, 1
+    key = other > key ? other : key;
+    other = __builtin_amdgcn_mov_dpp(key, 0x141, 0xf, 0xf, true);                // the half row mirrored
+    return other > key ? other : key;
+}
+
+// First launch of two, a wavefront per workgroup: a group is the 128 bytes that eight lanes read together
+// (of each of the workgroup's pieces), so that reading it again is reading a cache line.  Lane 8 i + j
+// keeps the maximum of the lanes 8 i .. 8 i + 7 in vector j.
+template <typename E, bool LSE> __global__ __launch_bounds__(64) void top_maxima(Top a)
+{
+    constexpr int kItems = E::items, kPiece = 64 * kPieceVecs * kItems;
+    const int64_t at = blockIdx.x / a.tiles, row = a.row0 + at;
+    const int tile = blockIdx.x % a.tiles, lane = threadIdx.x;
     const typename E::item *in = reinterpret_cast<const typename E::item *>(a.in + row * a.stride);
-    const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
+    int64_t first = (int64_t)tile * a.pieces * kPiece - nbh_row_before<E>(in);
     nbh_softmax stats = nbh_softmax_empty();
-    float peak[kAhead];
+    uint32_t mine = 0;
+    for (int piece = 0; piece < a.pieces && first < a.vocab; ++piece, first += kPiece) {
+        nbh_u32x4 raw[kPieceVecs];
+        const bool full = first >= 0 && first + kPiece <= a.vocab;
+        if (full) {
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-        peak[j] = -INFINITY;
-    nbh_row_stream<E, T, false>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kAhead]) __attribute__((always_inline)) {
+            for (int j = 0; j < kPieceVecs; ++j)
+                raw[j] = E::template load<true>(in + first + (j * 64 + lane) * kItems);
+        } else {
 #pragma unroll
-        for (int j = 0; j < kAhead; ++j) {
+            for (int j = 0; j < kPieceVecs; ++j)
+                raw[j] = nbh_row_load_raw<E, true>(in, first + (j * 64 + lane) * kItems, a.vocab, E::lowest);
+        }
+#pragma unroll
+        for (int j = 0; j < kPieceVecs; ++j) {
             float f[kItems];
             E::unpack(raw[j], f);
             const float most = nbh_row_most(f);
-            peak[j] = __builtin_elementwise_maximum(peak[j], most);
+            const int64_t v = first + (j * 64 + lane) * kItems;
+            uint32_t key = key_of(most);
+            if (!full && (v >= a.vocab || v + kItems <= 0))
+                key = 0;
+            key = most_of_eight(key);
+            if ((lane & 7) == j)
+                mine = key > mine ? key : mine;
             if (LSE)
                 nbh_softmax_add(stats, f, most, a.scale);
         }
-    });
-    uint32_t *out = a.maxima + (blockIdx.x * (int64_t)a.parts) * T + threadIdx.x;
-    uint32_t lane = 0;
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-        const uint32_t key = begin + (j * T + (int64_t)threadIdx.x) * kItems < end ? key_of(peak[j]) : 0u;
-        lane = key > lane ? key : lane;
-        if (a.parts > 1)
-            out[j * T] = key;
     }
-    if (a.parts == 1)
-        out[0] = lane;
+    a.maxima[blockIdx.x * (int64_t)64 + lane] = mine;
     if (LSE) {
-        stats = nbh_softmax_group<T>(stats, a.scale, room);
-        if (threadIdx.x == 0)
-            a.part_stats[at * a.splits + split] = stats;
+        stats = nbh_softmax_wave(stats, a.scale);
+        if (lane == 0)
+            a.part_stats[blockIdx.x] = stats;
     }
 }
 
-// Second launch: a workgroup per row, P groups per lane.
-template <typename E, bool LSE, int P> __global__ __launch_bounds__(kFinishThreads) void top_finish(Top a)
+// Second launch: a workgroup per row, up to P groups per lane.
+template <typename E, bool LSE, int T, int P, int CAP> __global__ __launch_bounds__(T) void top_finish(Top a)
 {
     typedef typename E::item item;
-    constexpr int T = kFinishThreads, kItems = E::items, M = kMaximaThreads, CAP = 4096;
-    constexpr int kChunk = kAhead * M * kItems;
+    constexpr int kItems = E::items, kPiece = 64 * kPieceVecs * kItems;
     __shared__ __align__(16) uint64_t list[CAP + 2];
     __shared__ int again[CAP];
     __shared__ Shared<T> sh;
     const int64_t row = a.row0 + blockIdx.x;
     const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
-    const int groups = a.splits * a.parts * M;
+    const int before = nbh_row_before<E>(in);
+    const int groups = a.tiles * 64;
     const uint32_t *maxima = a.maxima + blockIdx.x * (int64_t)groups;
     int turn = 0;
     if (threadIdx.x == 0)
@@ -413,81 +477,49 @@ template <typename E, bool LSE, int P> __global__ __launch_bounds__(kFinishThrea
         peaks[g] = at < groups ? maxima[at] : 0u;
     }
     if (LSE && threadIdx.x < 64) {
-        static_assert(kMostGroups / M <= 64, "a lane per stretch");
-        const int lane = threadIdx.x;
-        nbh_softmax stats = lane < a.splits ? a.part_stats[blockIdx.x * (int64_t)a.splits + lane] : nbh_softmax_empty();
-        for (int step = 32; step; step >>= 1) {
-            const nbh_softmax other = {__shfl_xor(stats.peak, step), __shfl_xor(stats.sum, step)};
-            stats = nbh_softmax_join(stats, other, a.scale);
-        }
-        if (lane == 0)
+        nbh_softmax stats = nbh_softmax_empty();
+        for (int s = threadIdx.x; s < a.tiles; s += 64)
+            stats = nbh_softmax_join(stats, a.part_stats[blockIdx.x * (int64_t)a.tiles + s], a.scale);
+        stats = nbh_softmax_wave(stats, a.scale);
+        if (threadIdx.x == 0)
             a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
-    uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
-    const int chunks = (int)(a.slice / kChunk), vectors = chunks * (a.parts > 1 ? 1 : kAhead);       // of a group
-    for (;;) {
-#pragma unroll
-        for (int g = 0; g < P; ++g)
-            if (peaks[g] && peaks[g] >= (uint32_t)(bound >> 32)) {
-                const int place = atomicAdd(&sh.groups, 1);
-                if (place < CAP)
-                    again[place] = g * T + threadIdx.x;
-            }
-        __syncthreads();
-        if (sh.groups <= CAP) {
-            for (int64_t i = threadIdx.x; i < (int64_t)sh.groups * vectors; i += T) {
-                const int g = again[i / vectors], v = (int)(i % vectors);
-                const int lane = g % M, part = g / M % a.parts, split = g / M / a.parts;
-                const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
-                const int64_t at = a.parts > 1 ? begin + v * (int64_t)kChunk + (part * M + lane) * kItems
-                                               : begin + (v * (int64_t)M + lane) * kItems;
-                append<E, T, CAP>(in, at, end, bound, list, sh);
-            }
-            __syncthreads();
-            if (sh.count <= CAP)
-                break;
-        }
-        bound = raised_bound<E, T, CAP>(in, a.vocab, (uint32_t)(bound >> 32), top, a.k, sh, turn);
-        __syncthreads();
-        if (threadIdx.x == 0)
-            sh.groups = sh.count = 0;
-        __syncthreads();
-    }
+    const uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
+    collect<E, T, CAP>(
+        in, a.vocab, bound, top, a.k, list, again, sh, turn, groups, 8 * a.pieces, [&](int g) { return maxima[g]; },
+        [&](int g, int v) {
+            const int64_t piece = (int64_t)(g / 64) * a.pieces + v / 8;
+            const int lane = g % 64 / 8 * 8 + v % 8, j = g % 8;
+            return piece * kPiece - before + (j * 64 + lane) * kItems;
+        });
     write_ranked<E, T>(a, row, list, sh.count);
 }
 
-// Workgroups per row: one from 256 rows on (a compute unit each), or where a row is a chunk or less; else
-// enough for four per compute unit, with at most kMostGroups groups.  Four groups per lane where k is more
-// than a quarter of the groups would otherwise be.
-struct Split {
-    int splits, parts;
-    int64_t slice;
+// Workgroups of the first launch per row and their pieces; 0 tiles: one launch.  `spare`: entries before a
+// row's beginning that its first vector may hold.
+// Two launches where a few workgroups would read long rows for themselves.  Measured, k = 50, one against
+// two: rows of 256 KiB, 1 row 17 and 16 us, 64 rows 19 and 18, 200 rows 20 and 23; rows of 512 KiB, 1 row 26
+// and 16, 64 rows 28 and 21, 200 rows 32 and 31; rows of 128 KiB, 1 row 13 and 16.
+struct Spread {
+    int tiles, pieces;
 };
-Split split_of(int64_t rows, int64_t vocab, int64_t k, int dtype)
+Spread spread_of(int64_t rows, int64_t vocab, int dtype, int spare)
 {
-    const int64_t chunk = (int64_t)kMaximaThreads * kAhead * (dtype == NBH_ROW_F32 ? 4 : 8);
-    const int64_t chunks = (vocab + chunk - 1) / chunk;
-    if (rows >= 256 || chunks == 1)
-        return {1, 1, vocab};
-    int64_t splits = (1024 + rows - 1) / rows;
-    if (splits > chunks)
-        splits = chunks;
-    if (splits > kMostGroups / kMaximaThreads)
-        splits = kMostGroups / kMaximaThreads;
-    int parts = k > splits * kMaximaThreads / 4 ? kAhead : 1;
-    if (parts * splits > kMostGroups / kMaximaThreads)
-        parts = 1;
-    const int64_t each = (chunks + splits - 1) / splits;
-    return {(int)((chunks + each - 1) / each), parts, each * chunk};
+    const int64_t piece = 64 * kPieceVecs * (dtype == NBH_ROW_F32 ? 4 : 8);
+    const int64_t all = (vocab + spare + piece - 1) / piece;
+    if (rows >= 128 || vocab <= 20 * piece)
+        return {0, 0};
+    const int64_t pieces = (all + kMostGroups / 64 - 1) / (kMostGroups / 64);
+    return {(int)((all + pieces - 1) / pieces), (int)pieces};
 }
 
 template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t stream)
 {
-    const int64_t most = NBH_ROW_MOST_GROUPS / a.splits;
+    const int64_t most = NBH_ROW_MOST_GROUPS / (a.tiles ? a.tiles : 1);
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
         const dim3 grid((unsigned)now);
-        if (a.splits == 1) {
+        if (a.tiles == 0) {
             // 256 lanes make 1024 groups, which serve up to k = 256; larger workgroups wait longer at
             // their barriers (4096 x 65536 bfloat16, k = 64: 124 us, with 512 lanes 140 us)
             if (a.k <= 256)
@@ -495,12 +527,13 @@ template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t 
             else
                 top_rows<E, LSE, 512, 4096><<<grid, dim3(512), 0, stream>>>(a);
         } else {
-            top_maxima<E, LSE><<<dim3((unsigned)(now * a.splits)), dim3(kMaximaThreads), 0, stream>>>(a);
-            const int groups = a.splits * a.parts * kMaximaThreads;
-            if (groups <= 8 * kFinishThreads)
-                top_finish<E, LSE, 8><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
+            top_maxima<E, LSE><<<dim3((unsigned)(now * a.tiles)), dim3(64), 0, stream>>>(a);
+            if (a.tiles * 64 > 4096)
+                top_finish<E, LSE, 512, kMostGroups / 512, 4096><<<grid, dim3(512), 0, stream>>>(a);
+            else if (a.k > 128)
+                top_finish<E, LSE, 512, 8, 4096><<<grid, dim3(512), 0, stream>>>(a);
             else
-                top_finish<E, LSE, kMostGroups / kFinishThreads><<<grid, dim3(kFinishThreads), 0, stream>>>(a);
+                top_finish<E, LSE, 256, 16, 1024><<<grid, dim3(256), 0, stream>>>(a);
         }
         if (const int status = nbh_launch_status())
             return status;
@@ -519,10 +552,8 @@ extern "C" size_t nbh_rows_top_workspace(int64_t rows, int64_t vocab, int64_t k,
     if (rows <= 0 || vocab <= 0 || vocab > INT32_MAX || k <= 0 || k > vocab || k > NBH_ROW_TOP_MOST || dtype < 0 ||
         dtype > NBH_ROW_BF16)
         return 0;
-    const Split s = split_of(rows, vocab, k, dtype);
-    return s.splits == 1 ? 0
-                         : (size_t)rows * s.splits *
-                               ((size_t)s.parts * kMaximaThreads * sizeof(uint32_t) + sizeof(nbh_softmax));
+    const Spread s = spread_of(rows, vocab, dtype, 7);
+    return (size_t)rows * s.tiles * (64 * sizeof(uint32_t) + sizeof(nbh_softmax));
 }
 
 extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int64_t stride, int dtype, int64_t k,
@@ -536,7 +567,7 @@ extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int
         return 0;
     if (!logits || !values || !indices)
         return (int)hipErrorInvalidValue;
-    const Split split = split_of(rows, vocab, k, dtype);
+    const Spread spread = spread_of(rows, vocab, dtype, nbh_row_spare(logits, stride, dtype));
     const size_t need = nbh_rows_top_workspace(rows, vocab, k, dtype);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
         return (int)hipErrorInvalidValue;
@@ -552,11 +583,10 @@ extern "C" int nbh_rows_top(const void *logits, int64_t rows, int64_t vocab, int
     a.lse = lse;
     a.temperature = (float)temperature;
     a.scale = (float)(1.4426950408889634 / a.temperature);
-    a.splits = split.splits;
-    a.parts = split.parts;
-    a.slice = split.slice;
+    a.tiles = spread.tiles;
+    a.pieces = spread.pieces;
     a.maxima = (uint32_t *)workspace;
-    a.part_stats = (nbh_softmax *)(a.maxima + (size_t)rows * split.splits * split.parts * kMaximaThreads);
+    a.part_stats = (nbh_softmax *)(a.maxima + (size_t)rows * spread.tiles * 64);
 
     const hipStream_t s = nbh_hip_stream(stream);
     nbh_stream_report report(s);

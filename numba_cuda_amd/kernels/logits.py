@@ -36,20 +36,32 @@ MOST = 1024                                  # NBH_ROW_TOP_MOST: entries `top` r
 
 _F32, _F16, _BF16 = 0, 1, 2                  # enum nbh_row_dtype
 _LOSS, _GRAD = 1, 2                          # enum nbh_distill_what
-_float32, _int32, _int64 = np.dtype(np.float32), np.dtype(np.int32), np.dtype(np.int64)
-_ROW_DTYPE = {_float32: _F32, np.dtype(np.float16): _F16, bfloat16: _BF16}
+_float32, _float16 = np.dtype(np.float32), np.dtype(np.float16)
+_int32, _int64, _uint32 = np.dtype(np.int32), np.dtype(np.int64), np.dtype(np.uint32)
 
 _ADJUST = struct.Struct("@qPP6q3P4q3P3d3P3qPq")       # struct nbh_logits_adjust_args
 _DISTILL = struct.Struct("@qqP4q2P5q2Pqdd3PqPq")      # struct nbh_rows_distill_args
 
 
 # ---- arguments ---------------------------------------------------------------------------
+#
+# A call of a few microseconds on the device should not take many on the host.  An argument becomes a
+# row view (address, rows, columns, bytes from row to row, code) or a vector view (address, items, item
+# size), for ordinary ones in one native call (row_view / vector_view of _hostbuf, which go by these
+# tables); whatever that declines takes the path through _device_view, which also raises what there is
+# to raise.  Class -> are its strides counted in items; dtype object -> (item size, code).  The classes
+# and dtype objects of torch are added when the first of them is seen.
+_ROWS = {devicearray.DeviceNDArray: False, _float32: (4, _F32), _float16: (2, _F16), bfloat16: (2, _BF16)}
+_INTEGER_ROWS = {devicearray.DeviceNDArray: False, _int32: (4, 4), _int64: (8, 8)}
+_INT32_ROWS = {devicearray.DeviceNDArray: False, _int32: (4, 4)}
+_WORDS = {devicearray.DeviceNDArray: False, _int32: (4, 0), _uint32: (4, 0)}
+_INTEGERS = {devicearray.DeviceNDArray: False, _int32: (4, 4), _int64: (8, 8)}
+_FLOATS = {devicearray.DeviceNDArray: False, _float32: (4, 0)}
+_TABLES = (_ROWS, _INTEGER_ROWS, _INT32_ROWS, _WORDS, _INTEGERS, _FLOATS)
 
-# A call of a few microseconds on the device should not take many on the host: arguments become plain
-# tuples (address, shape, byte strides, dtype, what keeps the memory alive), found by the class of the
-# argument; a torch tensor's attributes cost a tenth of what its interface dictionary does.
+_row_view, _vector_view = _driver._hostbuf.row_view, _driver._hostbuf.vector_view
 
-_foreign_dtypes = {}                         # dtype objects of other libraries -> (np.dtype, its item size)
+_foreign_dtypes = {}                         # dtype objects of other libraries -> np.dtype
 
 
 def _foreign_dtype(dtype):
@@ -58,172 +70,137 @@ def _foreign_dtype(dtype):
         found = bfloat16 if name == "bfloat16" else np.dtype(name)
     except TypeError:
         raise TypeError("unsupported dtype: %s" % (dtype,)) from None
-    _foreign_dtypes[dtype] = found, found.itemsize
-    return _foreign_dtypes[dtype]
+    _foreign_dtypes[dtype] = found
+    for table in _TABLES:
+        if found in table:
+            table[dtype] = table[found]
+    return found
 
 
-def _view_of_own(array):
-    try:
-        address = array.gpu_data.device_pointer
-    except AttributeError:
-        address = array.device_ctypes_pointer.value or 0
-    return address, array.shape, array.strides, array.dtype, array
-
-
-def _view_of_tensor(tensor):
-    if not tensor.is_cuda:
-        return None
-    dtype = tensor.dtype
-    dtype, size = _foreign_dtypes.get(dtype) or _foreign_dtype(dtype)
-    strides = tensor.stride()
-    if len(strides) == 1:
-        strides = (strides[0] * size,)
-    elif len(strides) == 2:
-        strides = (strides[0] * size, strides[1] * size)
-    else:
-        strides = tuple([n * size for n in strides])
-    return tensor.data_ptr(), tensor.shape, strides, dtype, tensor
-
-
-_views = {devicearray.DeviceNDArray: _view_of_own}       # class -> function
+def _is_tensor(obj):
+    if not (hasattr(obj, "is_cuda") and hasattr(obj, "data_ptr") and hasattr(obj, "stride")):
+        return False
+    if type(obj).__name__ == "Tensor":       # not its subclasses
+        for table in _TABLES:
+            table[type(obj)] = True
+    return True
 
 
 def _device_view(obj):
-    """The tuple of something in device memory, None for anything else."""
-    view = _views.get(obj.__class__)
-    if view is not None:
-        return view(obj)
+    """(address, shape, byte strides, dtype, what keeps it alive) of something in device memory, None
+    for anything else."""
     if getattr(obj, "__cuda_ndarray__", False):
-        return _view_of_own(obj)
-    if hasattr(obj, "is_cuda") and hasattr(obj, "data_ptr") and hasattr(obj, "stride"):
-        _views[obj.__class__] = _view_of_tensor
-        return _view_of_tensor(obj)
+        return obj.device_ctypes_pointer.value or 0, tuple(obj.shape), tuple(obj.strides), obj.dtype, obj
+    if _is_tensor(obj):
+        if not obj.is_cuda:
+            return None
+        dtype = _foreign_dtypes.get(obj.dtype) or _foreign_dtype(obj.dtype)
+        return obj.data_ptr(), tuple(obj.shape), tuple([n * dtype.itemsize for n in obj.stride()]), dtype, obj
     if hasattr(obj, "__cuda_array_interface__"):
-        return _view_of_own(devicearray.auto_device(obj)[0])
+        return _device_view(devicearray.auto_device(obj)[0])
     return None
 
 
 _several_devices = None
 
 
-def _check_device(view, name):
-    """Refuse memory of another device than the calling thread's."""
+def _one_device():
     global _several_devices
     if _several_devices is None:
         _several_devices = _driver.driver.get_device_count() > 1
-    if _several_devices and view[0]:
+    return not _several_devices
+
+
+def _checked_view(obj, name, stream, dtype=None, output=False):
+    """_device_view of an argument; an input on the host is copied over."""
+    view = _device_view(obj)
+    if view is None:
+        if output:
+            raise TypeError("%s must be a device array" % name)
+        host = np.ascontiguousarray(obj, dtype=dtype)
+        view = _device_view(devicearray.auto_device(host, stream=stream)[0])
+    if not _one_device() and view[0]:        # memory of another device than the calling thread's
         where, here = ctypes.c_int(), ctypes.c_int()
         _driver.driver.nbh_get_device(ctypes.byref(here))
         _driver.driver.nbh_pointer_device(view[0], ctypes.byref(where))
         if where.value != here.value:
             raise ValueError("%s is on device %d, the current device is %d" % (name, where.value, here.value))
-
-
-def _input(obj, name, stream, dtype=None):
-    """The tuple of an input; what is on the host is copied over."""
-    view = _device_view(obj)
-    if view is None:
-        host = np.asarray(obj) if dtype is None else np.asarray(obj, dtype=dtype)
-        if not host.flags["C_CONTIGUOUS"]:
-            host = np.ascontiguousarray(host)
-        view = _device_view(devicearray.auto_device(host, stream=stream)[0])
-    if _several_devices is not False:
-        _check_device(view, name)
     return view
 
 
-def _output(obj, name):
-    view = _device_view(obj)
-    if view is None:
-        raise TypeError("%s must be a device array" % name)
-    if _several_devices is not False:
-        _check_device(view, name)
-    return view
-
-
-def _as_rows(view, name, shape=None, dtypes=_ROW_DTYPE):
-    """Check a 2-d operand; returns the bytes from row to row."""
-    address, own_shape, strides, dtype, _ = view
-    if len(own_shape) != 2:
-        raise ValueError("%s must be a 2-d array, got %d-d" % (name, len(own_shape)))
-    if dtype not in dtypes:
+def _rows_of(obj, name, stream, table=_ROWS, output=False, keep=None):
+    """The row view of a 2-d argument; what a copy from the host needs alive goes into `keep`."""
+    if _several_devices is False:
+        view = _row_view(obj, table)
+        if view is not None:
+            return view
+    address, shape, strides, dtype, owner = _checked_view(obj, name, stream, output=output)
+    if len(shape) != 2:
+        raise ValueError("%s must be a 2-d array, got %d-d" % (name, len(shape)))
+    if dtype not in table:
         raise TypeError("%s has unsupported dtype %s" % (name, dtype))
-    if shape is not None and own_shape != shape:
-        raise ValueError("%s has shape %s, expected %s" % (name, tuple(own_shape), tuple(shape)))
-    size = dtype.itemsize
-    rows, columns = own_shape
+    size, code = table[dtype]
+    rows, columns = shape
     if columns > 1 and strides[1] != size:
         raise ValueError("the items of a row of %s must lie next to each other (strides %s)" % (name, strides))
     if address % size or (rows > 1 and strides[0] % size):
         raise ValueError("%s is not aligned to its item size" % name)
-    return strides[0] if rows > 1 else 0
+    if keep is not None:
+        keep.append(owner)
+    return address, rows, columns, strides[0] if rows > 1 else 0, code
 
 
-def _as_result_rows(view, name, shape, dtypes=_ROW_DTYPE):
-    stride = _as_rows(view, name, shape, dtypes)
-    if shape[0] > 1 and shape[1] and abs(stride) < shape[1] * view[3].itemsize:
-        raise ValueError("the rows of %s overlap (strides %s)" % (name, view[2]))
-    return stride
-
-
-def _as_vector(view, name, length, dtypes):
-    address, shape, strides, dtype, _ = view
+def _vector_of(obj, name, length, stream, table, dtype=None, output=False, keep=None):
+    """The vector view of a 1-d argument of `length` items (None: any number)."""
+    if _several_devices is False:
+        view = _vector_view(obj, table, -1 if length is None else length)
+        if view is not None:
+            return view
+    address, shape, strides, dtype, owner = _checked_view(obj, name, stream, dtype, output)
     if len(shape) != 1:
         raise ValueError("%s must be a 1-d array, got %d-d" % (name, len(shape)))
-    if dtype not in dtypes:
+    if dtype not in table:
         raise TypeError("%s has unsupported dtype %s" % (name, dtype))
-    n = shape[0]
+    size, n = dtype.itemsize, shape[0]
     if length is not None and n != length:
         raise ValueError("%s has %d items, expected %d" % (name, n, length))
-    size = dtype.itemsize
     if n > 1 and strides[0] != size:
         raise ValueError("%s must have unit stride" % name)
     if address % size:
         raise ValueError("%s is not aligned to its item size" % name)
-    return view
+    if keep is not None:
+        keep.append(owner)
+    return address, n, size
 
 
-_INTEGERS = (_int32, _int64)
-_FLOATS = (_float32,)
-
-
-def _extent(view):
-    """First and last + 1 address of the items."""
-    low, shape, strides, dtype, _ = view
-    high = low
-    for n, step in zip(shape, strides):
-        if n == 0:
-            return low, low
-        if step < 0:
-            low += (n - 1) * step
-        else:
-            high += (n - 1) * step
-    return low, high + dtype.itemsize
+_SIZE = (4, 2, 2)                            # item size by row code
 
 
 def _refuse_overlaps(results, inputs, same=None):
-    """ValueError when a result array touches an input or another result; `same`: the input that a
-    result may be, item for item.  Both are lists of (tuple, name)."""
-    spans = [(*_extent(view), view, name) for view, name in results]
-    others = spans + [(*_extent(view), view, name) for view, name in inputs]
-    for at, (low, high, out, name) in enumerate(spans):
-        for other_low, other_high, other, other_name in others[at + 1:]:
+    """ValueError when a result array touches an input or another result.  Both are lists of blocks
+    (address, rows, bytes of a row, bytes from row to row, name); `same`: the input that a result may
+    be, byte for byte."""
+    spans = []
+    for block in results + inputs:
+        address, rows, width, step, _ = block
+        reach = (rows - 1) * step
+        low, high = (address + reach, address + width) if reach < 0 else (address, address + reach + width)
+        spans.append((low, high if rows and width else low, block))
+    for at, (low, high, out) in enumerate(spans[:len(results)]):
+        for other_low, other_high, other in spans[at + 1:]:
             if low < other_high and other_low < high and low < high and other_low < other_high and not (
-                    other is same and _same_items(out, other)) and not _beside(out, other):
-                raise ValueError("%s overlaps %s" % (name, other_name))
-
-
-def _same_items(out, other):
-    return out[0] == other[0] and out[3] == other[3] and (out[1][0] <= 1 or out[2][0] == other[2][0])
+                    other is same and out[:3] == other[:3] and (out[1] <= 1 or out[3] == other[3])) and not _beside(
+                    out, other):
+                raise ValueError("%s overlaps %s" % (out[4], other[4]))
 
 
 def _beside(out, other):
     """Columns of one wider buffer lie between each other without touching."""
-    if len(out[1]) == len(other[1]) == 2 and out[2][0] == other[2][0] > 0:
-        pitch = out[2][0]
-        gap = (other[0] - out[0]) % pitch
-        return gap >= out[1][1] * out[3].itemsize and gap + other[1][1] * other[3].itemsize <= pitch
-    return False
+    pitch = out[3]
+    if pitch != other[3] or pitch <= 0:
+        return False
+    gap = (other[0] - out[0]) % pitch
+    return gap >= out[2] and gap + other[2] <= pitch
 
 
 def _number(value, name, low=None, high=None):
@@ -257,26 +234,36 @@ def _new(shape, dtype, stream, handle, name):
     return devicearray.DeviceNDArray(shape, strides, dtype, stream=stream)
 
 
-def _result(obj, name, shape, dtype, stream, handle):
-    """(what the caller gets back, its tuple) for a result that may have been given."""
+def _result_rows(obj, name, rows, columns, dtype, stream, handle, table=_ROWS):
+    """(what the caller gets back, its row view) for a rows x columns result that may have been given."""
+    if obj is None:
+        obj = _new((rows, columns), dtype, stream, handle, name)
+    view = _rows_of(obj, name, stream, table, output=True)
+    if view[1] != rows or view[2] != columns:
+        raise ValueError("%s has shape %s, expected %s" % (name, view[1:3], (rows, columns)))
+    if rows > 1 and columns and abs(view[3]) < columns * (_SIZE[view[4]] if table is _ROWS else view[4]):
+        raise ValueError("the rows of %s overlap (%d bytes from one to the next)" % (name, view[3]))
+    return obj, view
+
+
+def _result_numbers(obj, name, rows, stream, handle):
     if obj is None or obj is True:
-        obj = _new(shape, dtype, stream, handle, name)
-    return obj, _output(obj, name)
+        obj = _new((rows,), _float32, stream, handle, name)
+    return obj, _vector_of(obj, name, rows, stream, _FLOATS, output=True)[0]
 
 
 def _workspace(given, nbytes, handle):
     """(address, bytes, what keeps it alive)."""
     if given is not None:
-        view = _output(given, "workspace")
-        low, high = _extent(view)
-        items = 1
-        for n in view[1]:
-            items *= n
-        if items * view[3].itemsize != high - low:
-            raise ValueError("workspace must be contiguous")
-        if high - low < nbytes or low % 16:
+        address, shape, strides, dtype, owner = _checked_view(given, "workspace", 0, output=True)
+        expect = dtype.itemsize
+        for n, step in zip(shape[::-1], strides[::-1]):
+            if n > 1 and step != expect:
+                raise ValueError("workspace must be contiguous")
+            expect *= n
+        if expect < nbytes or address % 16:
             raise ValueError("workspace must hold %d bytes, aligned to 16" % nbytes)
-        return low, high - low, view[4]
+        return address, expect, owner
     if not nbytes:
         return _NO_WORKSPACE
     if _capturing(handle):
@@ -289,17 +276,16 @@ _NO_WORKSPACE = (0, 0, None)
 
 # ---- penalties, biases, masks --------------------------------------------------------------
 
-def _per_row(value, name, rows, stream, number):
-    """(address, value in its place, what keeps it alive) of a number or one number per row."""
+def _per_row(value, name, rows, stream, number, keep):
+    """(address, value in its place) of a number or one number per row."""
     if value is None:
-        return 0, number, None
+        return 0, number
     if _is_number(value):
         value = _number(value, name)
         if name == "repetition" and value <= 0:
             raise ValueError("repetition must be positive, got %r" % value)
-        return 0, value, None
-    view = _as_vector(_input(value, name, stream, np.float32), name, rows, _FLOATS)
-    return view[0], number, view[4]
+        return 0, value
+    return _vector_of(value, name, rows, stream, _FLOATS, np.float32, keep=keep)[0], number
 
 
 def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, repetition=None, presence=None,
@@ -321,10 +307,8 @@ def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, 
     """
     devices.get_context()
     handle = _driver._stream_handle(stream)
-    x = _input(logits, "logits", stream)
-    in_stride = _as_rows(x, "logits")
-    shape, dtype = x[1], x[3]
-    rows, vocab = shape
+    keep = []                                # copies of host arrays, alive until the launch is made
+    address, rows, vocab, in_stride, code = _rows_of(logits, "logits", stream, keep=keep)
     if (tokens is None) != (offsets is None):
         raise ValueError("tokens and offsets come together")
     if tokens is None and not (prompt_lengths is repetition is presence is frequency is None):
@@ -332,55 +316,65 @@ def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, 
     if (bias_tokens is None) != (bias_values is None) or (bias_tokens is None) != (bias_offsets is None):
         raise ValueError("bias_tokens, bias_values and bias_offsets come together")
 
-    out, y = _result(out, "out", shape, dtype, stream, handle)
-    out_stride = _as_result_rows(y, "out", shape)
-    if y[3] != dtype and y[3] != _float32:
-        raise TypeError("out has dtype %s, expected %s or float32" % (y[3], dtype))
-    _refuse_overlaps([(y, "out")], [(x, "logits")], same=x)
+    out, y = _result_rows(out, "out", rows, vocab, _DTYPE[code], stream, handle)
+    if y[4] != code and y[4] != _F32:
+        raise TypeError("out has dtype %s, expected %s or float32" % (_DTYPE[y[4]], _DTYPE[code]))
+    x = (address, rows, vocab * _SIZE[code], in_stride, "logits")
+    _refuse_overlaps([(y[0], rows, vocab * _SIZE[y[4]], y[3], "out")], [x], same=x)
 
-    t = o = p = rep = pre = fre = bt = bo = bv = m = None        # alive until the launch is made
     history, bias = _NO_HISTORY, _NO_BIAS
     if tokens is not None:
-        t = _as_vector(_input(tokens, "tokens", stream), "tokens", None, _INTEGERS)
-        o = _as_vector(_input(offsets, "offsets", stream), "offsets", rows + 1, _INTEGERS)
+        t = _vector_of(tokens, "tokens", None, stream, _INTEGERS, keep=keep)
+        o = _vector_of(offsets, "offsets", rows + 1, stream, _INTEGERS, keep=keep)
         p = _NO_PROMPTS
         if prompt_lengths is not None:
-            p = _as_vector(_input(prompt_lengths, "prompt_lengths", stream), "prompt_lengths", rows, _INTEGERS)
-        rep = _per_row(repetition, "repetition", rows, stream, 1.0)
-        pre = _per_row(presence, "presence", rows, stream, 0.0)
-        fre = _per_row(frequency, "frequency", rows, stream, 0.0)
-        history = (t[0], o[0], p[0], t[1][0], t[3].itemsize, o[3].itemsize, p[3].itemsize, rep[0], pre[0], fre[0],
-                   rep[1], pre[1], fre[1])
+            p = _vector_of(prompt_lengths, "prompt_lengths", rows, stream, _INTEGERS, keep=keep)
+        rep = _per_row(repetition, "repetition", rows, stream, 1.0, keep)
+        pre = _per_row(presence, "presence", rows, stream, 0.0, keep)
+        fre = _per_row(frequency, "frequency", rows, stream, 0.0, keep)
+        history = (t[0], o[0], p[0], t[1], t[2], o[2], p[2], rep[0], pre[0], fre[0], rep[1], pre[1], fre[1])
     if bias_tokens is not None:
-        bt = _as_vector(_input(bias_tokens, "bias_tokens", stream), "bias_tokens", None, _INTEGERS)
-        bv = _as_vector(_input(bias_values, "bias_values", stream, np.float32), "bias_values", bt[1][0], _FLOATS)
-        bo = _as_vector(_input(bias_offsets, "bias_offsets", stream), "bias_offsets", rows + 1, _INTEGERS)
-        bias = (bt[0], bo[0], bv[0], bt[1][0], bt[3].itemsize, bo[3].itemsize)
+        t = _vector_of(bias_tokens, "bias_tokens", None, stream, _INTEGERS, keep=keep)
+        v = _vector_of(bias_values, "bias_values", t[1], stream, _FLOATS, np.float32, keep=keep)
+        o = _vector_of(bias_offsets, "bias_offsets", rows + 1, stream, _INTEGERS, keep=keep)
+        bias = (t[0], o[0], v[0], t[1], t[2], o[2])
     mask_address = mask_stride = 0
     if mask is not None:
-        m = _input(mask, "mask", stream)
-        mask_address, mask_shape, mask_strides, mask_dtype, _ = m
-        if mask_dtype.kind not in "iu" or mask_dtype.itemsize != 4:
-            raise TypeError("mask has dtype %s, expected 32-bit integers" % mask_dtype)
-        if len(mask_shape) not in (1, 2) or (len(mask_shape) == 2 and mask_shape[0] not in (1, rows)):
-            raise ValueError("mask has shape %s, expected one row of words or %d" % (tuple(mask_shape), rows))
-        words = mask_shape[-1]
-        if words * 32 < vocab:
-            raise ValueError("mask has %d words, %d entries need %d" % (words, vocab, -(-vocab // 32)))
-        if words > 1 and mask_strides[-1] != 4:
-            raise ValueError("the words of a mask must lie next to each other (strides %s)" % (mask_strides,))
-        if len(mask_shape) == 2 and mask_shape[0] > 1:
-            mask_stride = mask_strides[0]
+        mask_address, mask_stride = _mask_of(mask, rows, vocab, stream, keep)
 
     if rows and vocab:
         _driver.driver.nbh_logits_adjust(
-            _ADJUST.pack(_ADJUST_SIZE, x[0], y[0], rows, vocab, in_stride, out_stride, _ROW_DTYPE[dtype],
-                         _ROW_DTYPE[y[3]], *history, *bias, mask_address, mask_stride), handle or None)
+            _ADJUST.pack(_ADJUST_SIZE, address, y[0], rows, vocab, in_stride, y[3], code, y[4], *history, *bias,
+                         mask_address, mask_stride), handle or None)
     return out
 
 
+def _mask_of(mask, rows, vocab, stream, keep):
+    """(address, bytes from row to row) of the words of a mask."""
+    view = _row_view(mask, _WORDS) if _several_devices is False else None
+    if view is not None:
+        address, masks, words, stride, _ = view
+    else:
+        address, shape, strides, dtype, owner = _checked_view(mask, "mask", stream)
+        keep.append(owner)
+        if dtype not in _WORDS:
+            raise TypeError("mask has dtype %s, expected 32-bit integers" % dtype)
+        if len(shape) not in (1, 2):
+            raise ValueError("mask has shape %s, expected one row of words or %d" % (shape, rows))
+        words, masks = shape[-1], shape[0] if len(shape) == 2 else 1
+        if words > 1 and strides[-1] != 4:
+            raise ValueError("the words of a mask must lie next to each other (strides %s)" % (strides,))
+        stride = strides[0] if masks > 1 else 0
+    if masks != rows and masks != 1:
+        raise ValueError("mask has shape %s, expected one row of words or %d" % ((masks, words), rows))
+    if words * 32 < vocab:
+        raise ValueError("mask has %d words, %d entries need %d" % (words, vocab, -(-vocab // 32)))
+    return address, stride if masks > 1 else 0
+
+
+_DTYPE = (_float32, _float16, bfloat16)      # by code
 _ADJUST_SIZE = _ADJUST.size
-_NO_PROMPTS = (0, (0,), (4,), _int32, None)
+_NO_PROMPTS = (0, 0, 4)
 _NO_HISTORY = (0, 0, 0, 0, 4, 4, 4, 0, 0, 0, 1.0, 0.0, 0.0)
 _NO_BIAS = (0, 0, 0, 0, 4, 4)
 
@@ -397,11 +391,11 @@ def _count(k, most):
 
 def _row_code(dtype):
     if str(dtype).startswith("torch."):
-        dtype = _foreign_dtype(dtype)[0]
+        dtype = _foreign_dtype(dtype)
     dtype = np.dtype(dtype)
-    if dtype not in _ROW_DTYPE:
+    if dtype not in _DTYPE:
         raise TypeError("unsupported dtype %s" % dtype)
-    return _ROW_DTYPE[dtype]
+    return _DTYPE.index(dtype)
 
 
 def top_workspace(rows, vocab, k, dtype):
@@ -422,29 +416,24 @@ def top(logits, k, *, values=None, indices=None, lse=None, temperature=1.0, work
     """
     devices.get_context()
     handle = _driver._stream_handle(stream)
-    x = _input(logits, "logits", stream)
-    stride = _as_rows(x, "logits")
-    (rows, vocab), dtype = x[1], x[3]
+    keep = []
+    address, rows, vocab, stride, code = _rows_of(logits, "logits", stream, keep=keep)
     k = _count(k, min(vocab, MOST))
     temperature = _temperature(temperature)
-    shape = (rows, k)
-    values, v = _result(values, "values", shape, dtype, stream, handle)
-    values_stride = _as_result_rows(v, "values", shape, (dtype,))
-    indices, i = _result(indices, "indices", shape, _int32, stream, handle)
-    indices_stride = _as_result_rows(i, "indices", shape, (_int32,))
-    results, lse_address = [(v, "values"), (i, "indices")], None
-    wanted = lse is not None and lse is not False
+    values, v = _result_rows(values, "values", rows, k, _DTYPE[code], stream, handle)
+    if v[4] != code:
+        raise TypeError("values has dtype %s, expected %s" % (_DTYPE[v[4]], _DTYPE[code]))
+    indices, i = _result_rows(indices, "indices", rows, k, _int32, stream, handle, _INT32_ROWS)
+    results = [(v[0], rows, k * _SIZE[code], v[3], "values"), (i[0], rows, k * 4, i[3], "indices")]
+    lse_address, wanted = None, lse is not None and lse is not False
     if wanted:
-        lse, z = _result(lse, "lse", (rows,), _float32, stream, handle)
-        _as_vector(z, "lse", rows, _FLOATS)
-        lse_address = z[0]
-        results.append((z, "lse"))
-    _refuse_overlaps(results, [(x, "logits")])
-    code = _ROW_DTYPE[dtype]
+        lse, lse_address = _result_numbers(lse, "lse", rows, stream, handle)
+        results.append((lse_address, 1, rows * 4, 0, "lse"))
+    _refuse_overlaps(results, [(address, rows, vocab * _SIZE[code], stride, "logits")])
     if rows:
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_top_workspace(rows, vocab, k, code), handle)
-        _driver.driver.nbh_rows_top(x[0], rows, vocab, stride, code, k, v[0], values_stride, i[0], indices_stride,
-                                    lse_address, temperature, space[0] or None, space[1], handle or None)
+        _driver.driver.nbh_rows_top(address, rows, vocab, stride, code, k, v[0], v[3], i[0], i[3], lse_address,
+                                    temperature, space[0] or None, space[1], handle or None)
     return (values, indices, lse) if wanted else (values, indices)
 
 
@@ -460,65 +449,71 @@ def distill_workspace(rows, vocab, k, dtype, *, loss=True, grad=False):
 def _distill(what, grad_loss, student, values, indices, temperature, teacher_lse, loss, lse, out, workspace, stream):
     devices.get_context()
     handle = _driver._stream_handle(stream)
-    x = _input(student, "student", stream)
-    stride = _as_rows(x, "student")
-    shape, dtype = x[1], x[3]
-    rows, vocab = shape
-    v = _input(values, "values", stream)
-    values_stride = _as_rows(v, "values")
-    i = _input(indices, "indices", stream)
-    indices_stride = _as_rows(i, "indices", v[1], _INTEGERS)
-    if v[1][0] != rows:
-        raise ValueError("values has %d rows, student has %d" % (v[1][0], rows))
-    k = v[1][1]
+    keep = []
+    address, rows, vocab, stride, code = _rows_of(student, "student", stream, keep=keep)
+    v = _rows_of(values, "values", stream, keep=keep)
+    i = _rows_of(indices, "indices", stream, _INTEGER_ROWS, keep=keep)
+    k = v[2]
+    if i[1] != v[1] or i[2] != k:
+        raise ValueError("indices has shape %s, expected %s" % (i[1:3], v[1:3]))
+    if v[1] != rows:
+        raise ValueError("values has %d rows, student has %d" % (v[1], rows))
     if k > MOST:
         raise ValueError("a row of values may hold %d entries, got %d" % (MOST, k))
     temperature = _temperature(temperature)
-    inputs, results = [(x, "student"), (v, "values"), (i, "indices")], []
+    x = (address, rows, vocab * _SIZE[code], stride, "student")
+    inputs = [x, (v[0], rows, k * _SIZE[v[4]], v[3], "values"), (i[0], rows, k * i[4], i[3], "indices")]
+    results = []
     teacher_address = grad_address = grad_stride = loss_address = out_address = out_stride = 0
     grad_value = 0.0
     if teacher_lse is not None:
-        t = _as_vector(_input(teacher_lse, "teacher_lse", stream, np.float32), "teacher_lse", rows, _FLOATS)
-        teacher_address = t[0]
-        inputs.append((t, "teacher_lse"))
+        teacher_address = _vector_of(teacher_lse, "teacher_lse", rows, stream, _FLOATS, np.float32, keep=keep)[0]
+        inputs.append((teacher_address, 1, rows * 4, 0, "teacher_lse"))
     if what & _GRAD:
         if _is_number(grad_loss):
             grad_value = _number(grad_loss, "grad_loss")
         else:
-            g = _input(grad_loss, "grad_loss", stream, np.float32)
-            grad_address, grad_shape, strides, grad_dtype, _ = g
-            if len(grad_shape) != 1 or grad_shape[0] != rows:
-                raise ValueError("grad_loss has shape %s, expected (%d,)" % (tuple(grad_shape), rows))
-            if grad_dtype != _float32:
-                raise TypeError("grad_loss has unsupported dtype %s" % grad_dtype)
-            grad_stride = strides[0]
-            if grad_address % 4 or grad_stride % 4:
-                raise ValueError("grad_loss is not aligned to its item size")
-            inputs.append((g, "grad_loss"))
+            grad_address, grad_stride = _grad_loss_of(grad_loss, rows, stream, keep)
+            inputs.append((grad_address, rows, 4, grad_stride, "grad_loss"))
     if what & _LOSS:
-        loss, l = _result(loss, "loss", (rows,), _float32, stream, handle)
-        loss_address = _as_vector(l, "loss", rows, _FLOATS)[0]
-        lse, z = _result(lse, "lse", (rows,), _float32, stream, handle)
-        _as_vector(z, "lse", rows, _FLOATS)
-        results += [(l, "loss"), (z, "lse")]
+        loss, loss_address = _result_numbers(loss, "loss", rows, stream, handle)
+        lse, lse_address = _result_numbers(lse, "lse", rows, stream, handle)
+        results += [(loss_address, 1, rows * 4, 0, "loss"), (lse_address, 1, rows * 4, 0, "lse")]
     else:
-        z = _as_vector(_input(lse, "lse", stream, np.float32), "lse", rows, _FLOATS)
-        inputs.append((z, "lse"))
+        lse_address = _vector_of(lse, "lse", rows, stream, _FLOATS, np.float32, keep=keep)[0]
+        inputs.append((lse_address, 1, rows * 4, 0, "lse"))
     if what & _GRAD:
-        out, y = _result(out, "out", shape, dtype, stream, handle)
-        out_address, out_stride = y[0], _as_result_rows(y, "out", shape, (dtype,))
-        results.append((y, "out"))
+        out, y = _result_rows(out, "out", rows, vocab, _DTYPE[code], stream, handle)
+        if y[4] != code:
+            raise TypeError("out has dtype %s, expected %s" % (_DTYPE[y[4]], _DTYPE[code]))
+        out_address, out_stride = y[0], y[3]
+        results.append((out_address, rows, vocab * _SIZE[code], out_stride, "out"))
     _refuse_overlaps(results, inputs, same=x)
 
     if rows:
-        code = _ROW_DTYPE[dtype]
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_distill_workspace(rows, vocab, k, code, what), handle)
         _driver.driver.nbh_rows_distill(
-            _DISTILL.pack(_DISTILL_SIZE, what, x[0], rows, vocab, stride, code, v[0], i[0], k, values_stride,
-                          _ROW_DTYPE[v[3]], indices_stride, i[3].itemsize, teacher_address, grad_address, grad_stride,
-                          grad_value, temperature, loss_address, z[0], out_address, out_stride, space[0], space[1]),
-            handle or None)
+            _DISTILL.pack(_DISTILL_SIZE, what, address, rows, vocab, stride, code, v[0], i[0], k, v[3], v[4], i[3], i[4],
+                          teacher_address, grad_address, grad_stride, grad_value, temperature, loss_address,
+                          lse_address, out_address, out_stride, space[0], space[1]), handle or None)
     return loss, lse, out
+
+
+def _grad_loss_of(grad_loss, rows, stream, keep):
+    """(address, stride): of any stride, 0 too."""
+    if _several_devices is False:
+        view = _vector_view(grad_loss, _FLOATS, rows)
+        if view is not None:
+            return view[0], 4
+    address, shape, strides, dtype, owner = _checked_view(grad_loss, "grad_loss", stream, np.float32)
+    keep.append(owner)
+    if shape != (rows,):
+        raise ValueError("grad_loss has shape %s, expected (%d,)" % (shape, rows))
+    if dtype not in _FLOATS:
+        raise TypeError("grad_loss has unsupported dtype %s" % dtype)
+    if address % 4 or strides[0] % 4:
+        raise ValueError("grad_loss is not aligned to its item size")
+    return address, strides[0]
 
 
 _DISTILL_SIZE = _DISTILL.size

@@ -75,7 +75,8 @@ def test_top(name, rows, vocab, k):
 
 
 @pytest.mark.parametrize("name", cases.DTYPES)
-@pytest.mark.parametrize("rows, vocab, k", [(8, 1001, 30), (8, 30011, 1), (8, 30011, 100), (8, 9000, 1024)])
+@pytest.mark.parametrize("rows, vocab, k", [(8, 1001, 30), (8, 30011, 1), (8, 30011, 100), (8, 9000, 1024),
+                                            (8, 100003, 1), (8, 100003, 100), (8, 100003, 700)])
 def test_top_of_special_rows(name, rows, vocab, k):
     cases.check_top(cuda, rows, vocab, name, k, kind="edge")
     cases.check_top(cuda, rows, vocab, name, k, kind="edge", temperature=0.7)
@@ -106,6 +107,19 @@ def test_top_of_rows_that_fill_the_list_again_and_again():
             want = logits64.top(x[r * 400:r * 400 + 1], k) if k == 64 else np.lexsort(
                 (np.arange(150000), -x[r * 400]))[None, :k]
             assert np.array_equal(got[r * 400:(r + 1) * 400], np.repeat(want, 400, 0))
+
+
+@pytest.mark.parametrize("vocab", [40000, 200000])
+@pytest.mark.parametrize("k", [1, 50, 600])
+def test_top_of_masked_rows(vocab, k):
+    """Fewer entries than asked for are left: the rest are the first of the masked ones."""
+    rng = np.random.default_rng(vocab + k)
+    for left in (0, 1, 30, k):
+        x = np.full((3, vocab), -np.inf, np.float32)
+        for r in range(3):
+            at = rng.permutation(vocab)[:left]
+            x[r, at] = rng.standard_normal(left)
+        cases.check_top(cuda, 3, vocab, "float32", k, data=x)
 
 
 def test_top_into_wider_arrays_and_their_surroundings():
@@ -288,7 +302,7 @@ def test_torch_tensors_and_offsets_past_32_bits():
 
 def test_recorded_into_a_graph_and_replayed():
     torch = pytest.importorskip("torch")
-    rows, vocab, k = 6, 30011, 20
+    rows, vocab, k = 6, 60011, 20                # rows long enough that both calls need a workspace
     x = torch.zeros(rows, vocab, device="cuda")
     tokens = torch.randint(0, vocab, (300,), device="cuda", dtype=torch.int32)
     offsets = torch.arange(rows + 1, device="cuda") * 50

@@ -138,19 +138,21 @@ def test_adjust_refusals(fake_gpu):
 
 
 def test_columns_beside_each_other_do_not_overlap():
-    def array(start, n, pitch=100, rows=3):
-        return 4096 + 4 * start, (rows, n), (4 * pitch, 4), np.dtype(np.float32), None
+    def block(start, n, pitch=100, rows=3, name="logits"):
+        return 4096 + 4 * start, rows, 4 * n, 4 * pitch, name
+
     def check(one, other, same=None):
-        logits._refuse_overlaps([(one, "out")], [(other, "logits")], same=same)
-    check(array(0, 40), array(40, 60))
-    check(array(40, 60), array(0, 40))
+        logits._refuse_overlaps([(*one[:4], "out")], [other], same=same)
+    check(block(0, 40), block(40, 60))
+    check(block(40, 60), block(0, 40))
     for start, n in ((39, 10), (0, 40), (30, 5), (90, 20)):
         with pytest.raises(ValueError, match="out overlaps logits"):
-            check(array(0, 40), array(start, n, rows=4))
-    x = array(0, 40)
-    check(array(0, 40), x, same=x)
-    with pytest.raises(ValueError):
-        check(array(0, 40, pitch=99), x, same=x)
+            check(block(0, 40), block(start, n, rows=4))
+    x = block(0, 40)
+    check(block(0, 40), x, same=x)
+    for other in (block(0, 40, pitch=99), block(0, 80), block(1, 40)):      # another pitch, type or start
+        with pytest.raises(ValueError):
+            check(other, x, same=x)
 
 
 def test_top_refusals(fake_gpu):
@@ -168,6 +170,7 @@ def test_top_refusals(fake_gpu):
         (TypeError, "unsupported dtype", (_i32(2, 40), 1), {}),
         (TypeError, "device array", (x, 1), dict(indices=np.zeros((2, 1), np.int32))),
         (TypeError, "unsupported dtype", (x, 1), dict(indices=cuda.to_device(np.zeros((2, 1), np.int64)))),
+        (TypeError, "values has dtype", (x, 1), dict(values=cuda.to_device(np.zeros((2, 1), np.float16)))),
         (ValueError, "expected", (x, 2), dict(values=_f32(2, 3))),
         (ValueError, "expected 2", (x, 2), dict(lse=_f32(3))),
         (ValueError, "values overlaps logits", (x, 2), dict(values=x[:, :2])),
@@ -196,7 +199,7 @@ def test_distill_refusals(fake_gpu):
         (ValueError, "grad_loss has shape", both, (_f32(3), x, v, i), {}),
         (ValueError, "grad_loss", both, (float("nan"), x, v, i), {}),
         (TypeError, "grad_loss", both, (i[:, 0], x, v, i), {}),
-        (TypeError, "unsupported dtype", both, (g, x, v, i), dict(out=cuda.to_device(np.zeros((2, 40), np.float16)))),
+        (TypeError, "out has dtype", both, (g, x, v, i), dict(out=cuda.to_device(np.zeros((2, 40), np.float16)))),
         (ValueError, "out overlaps values", both, (g, x, _f32(2, 40)[:, :3], i), dict(out=None)),
         (ValueError, "expected 2", grad, (g, x, v, i, _f32(3)), {}),
     ]
@@ -246,6 +249,6 @@ def test_the_entry_points_check_their_arguments():
     assert lib.nbh_rows_top(None, 0, 10, 40, 0, 11, None, 4, None, 4, None, 1.0, None, 0, None) != 0
     assert lib.nbh_rows_top(None, 0, 10, 40, 0, 1, None, 4, None, 4, None, 0.0, None, 0, None) != 0
     assert lib.nbh_rows_distill(logits._DISTILL.pack(8, *([0] * 24)), None) != 0
-    # a single row of a long vocabulary is split, many rows are not
-    assert lib.nbh_rows_top_workspace(1, 131072, 50, 0) > 0 == lib.nbh_rows_top_workspace(4096, 131072, 50, 0)
+    # long rows are spread over workgroups, short ones are not
+    assert lib.nbh_rows_top_workspace(1, 131072, 50, 0) > 0 == lib.nbh_rows_top_workspace(4096, 1000, 50, 0)
     assert lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 1) > 0 == lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 2)
