@@ -8,7 +8,8 @@
 //     counts.
 //   * The groups whose maximum reaches it, about k, are listed in LDS and read again, a vector per lane;
 //     what reaches it there is appended to another list, whose order does not matter, and that is sorted:
-//     short ones by counting how many entries exceed each, others by a bitonic network.
+//     short ones by counting how many entries exceed each, others by buckets of their values, or where
+//     those are too uneven by a bitonic network.
 //   * Where too many entries reach it (masses of equal ones, rows sorted by blocks) the bound is raised, once:
 //     by bisection over all entries, and if it ends on a value that too many share, to the first of them.
 // Short rows: one workgroup does all of that for a row.  Long ones: a first launch of small workgroups in the
@@ -127,17 +128,16 @@ __device__ uint32_t bound_of(const uint32_t (&peaks)[P], int k, Shared<T> &sh, i
     return low;
 }
 
-// Appends what reaches `bound` of the entries at .. at + items.
+// Appends what reaches `bound` of the entries at .. at + items, the 16 bytes `raw`.
 template <typename E, int T, int CAP>
-__device__ __forceinline__ void append(const typename E::item *in, int64_t at, int64_t end, uint64_t bound,
-                                       uint64_t *list, Shared<T> &sh)
+__device__ __forceinline__ void append(nbh_u32x4 raw, int64_t at, int64_t end, uint64_t bound, uint64_t *list,
+                                       Shared<T> &sh)
 {
-    if (at >= end || at + E::items <= 0)
-        return;
     float f[E::items];
-    nbh_row_load<E, false>(in, at, end, -INFINITY, f);
-    if (key_of(nbh_row_most(f)) < (uint32_t)(bound >> 32))
+    E::unpack(raw, f);
+    if (at >= end || at + E::items <= 0 || key_of(nbh_row_most(f)) < (uint32_t)(bound >> 32))
         return;
+#pragma unroll
     for (int i = 0; i < E::items; ++i) {
         const uint64_t entry = entry_of(f[i], at + i);
         if (entry >= bound && at + i >= 0 && at + i < end) {
@@ -219,38 +219,51 @@ __device__ uint64_t raised_bound(const typename E::item *in, int64_t n, uint32_t
     return (uint64_t)low << 32;          // not reached: the row holds k entries
 }
 
+// Lists group g to be read again.
+template <int T, int CAP> __device__ __forceinline__ void list_group(int g, int *again, Shared<T> &sh)
+{
+    const int at = atomicAdd(&sh.groups, 1);
+    if (at < CAP)
+        again[at] = g;
+}
+
 // Brings at least k and at most CAP entries that reach a bound into the list, sh.count of them: first those
 // that reach `bound`; if they turn out to be too many, those that reach a raised one, which are not.
-// `most(g)`: key of the maximum of group g, 0 for an empty one; `place(g, v)`: first entry of its vector v.
-template <typename E, int T, int CAP, typename Most, typename Place>
-__device__ void collect(const typename E::item *in, int64_t n, uint64_t bound, uint32_t top, int k, uint64_t *list,
-                        int *again, Shared<T> &sh, int &turn, int groups, int vectors, Most most, Place place)
+// `reaching(key)` lists the groups whose maxima reach the key; `place(g, v)`: first entry of vector v of
+// group g.  Code that a workgroup runs once costs the fetching of its instructions: small loops, not
+// unrolled ones.
+template <typename E, int T, int CAP, typename Reaching, typename Place>
+__device__ __forceinline__ void collect(const typename E::item *in, int64_t n, uint64_t bound, uint32_t top, int k,
+                                        uint64_t *list, int *again, Shared<T> &sh, int &turn, int groups, int vectors,
+                                        Reaching reaching, Place place)
 {
+#pragma unroll 1
     for (int attempt = 0; attempt < 2; ++attempt) {
-        for (int g = threadIdx.x; g < groups; g += T) {
-            const uint32_t key = most(g);
-            if (key && key >= (uint32_t)(bound >> 32)) {
-                const int at = atomicAdd(&sh.groups, 1);
-                if (at < CAP)
-                    again[at] = g;
-            }
-        }
+        reaching((uint32_t)(bound >> 32));
         __syncthreads();
         const int listed = sh.groups;
-        if (listed <= CAP) {
-            for (int64_t i = threadIdx.x; i < (int64_t)listed * vectors; i += T)
-                append<E, T, CAP>(in, place(again[i / vectors], (int)(i % vectors)), n, bound, list, sh);
-        } else if (attempt) {
-            // many groups share the raised bound's value, but few of their entries its indices
-            for (int g = threadIdx.x; g < groups; g += T) {
-                const uint32_t key = most(g);
-                if (key && key >= (uint32_t)(bound >> 32))
-                    for (int v = 0; v < vectors; ++v)
-                        append<E, T, CAP>(in, place(g, v), n, bound, list, sh);
+        // With the raised bound many groups may share its value, but few of their entries its indices:
+        // then all groups are gone through.
+        const bool all = listed > CAP;
+        if (!all || attempt) {
+            const uint32_t vecs = (uint32_t)(all ? groups : listed) * vectors;
+            // the next vector is on its way while the last is looked at
+            uint32_t i = threadIdx.x;
+            int64_t at = i < vecs ? place(all ? i / vectors : again[i / vectors], i % vectors) : n;
+            nbh_u32x4 raw = nbh_row_load_raw<E, false>(in, at, n, E::lowest);
+#pragma unroll 1
+            for (; i < vecs; i += T) {
+                const uint32_t next = i + T;
+                const int64_t ahead =
+                    next < vecs ? place(all ? next / vectors : again[next / vectors], next % vectors) : n;
+                const nbh_u32x4 coming = nbh_row_load_raw<E, false>(in, ahead, n, E::lowest);
+                append<E, T, CAP>(raw, at, n, bound, list, sh);
+                raw = coming;
+                at = ahead;
             }
         }
         __syncthreads();
-        if (attempt || (listed <= CAP && sh.count <= CAP))
+        if (attempt || (!all && sh.count <= CAP))
             return;
         bound = raised_bound<E, T, CAP>(in, n, (uint32_t)(bound >> 32), top, k, sh, turn);
         __syncthreads();
@@ -260,10 +273,101 @@ __device__ void collect(const typename E::item *in, int64_t n, uint64_t bound, u
     }
 }
 
+// Ranks the list's entries by counting them into 1024 buckets of equal width between the smallest and the
+// largest key: put(rank, entry).  False, and nothing done, where a bucket is too crowded to be searched.
+// `counts` holds 1024 integers; the list's order changes.
+constexpr int kBuckets = 1024, kCrowd = 64;
+template <int T, int CAP, typename F>
+__device__ bool rank_by_buckets(uint64_t *list, int have, int *counts, Shared<T> &sh, F put)
+{
+    constexpr int kEach = CAP / T, kOf = kBuckets / T;
+    uint64_t mine[kEach];
+    uint32_t low = ~0u, high = 0;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        const int at = i * T + threadIdx.x;
+        mine[i] = at < have ? list[at] : 0;
+        const uint32_t key = (uint32_t)(mine[i] >> 32);
+        if (at < have) {
+            low = key < low ? key : low;
+            high = key > high ? key : high;
+        }
+    }
+    for (int step = 32; step; step >>= 1) {
+        const uint32_t l = __shfl_xor(low, step), h = __shfl_xor(high, step);
+        low = l < low ? l : low;
+        high = h > high ? h : high;
+    }
+    if ((threadIdx.x & 63) == 0) {
+        sh.ends[0][threadIdx.x >> 6] = high;
+        sh.ends[1][threadIdx.x >> 6] = low;
+    }
+    for (int i = threadIdx.x; i < kBuckets; i += T)
+        counts[i] = 0;
+    __syncthreads();
+    for (int w = 0; w < T / 64; ++w) {
+        high = sh.ends[0][w] > high ? sh.ends[0][w] : high;
+        low = sh.ends[1][w] < low ? sh.ends[1][w] : low;
+    }
+    const int bits = 32 - __clz((int)(high - low)), shift = bits > 10 ? bits - 10 : 0;
+    int place[kEach];                    // of an entry within its bucket
+    bool crowded = false;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i]) {
+            place[i] = atomicAdd(&counts[((uint32_t)(mine[i] >> 32) - low) >> shift], 1);
+            crowded |= place[i] >= kCrowd;
+        }
+    if (__syncthreads_or(crowded))
+        return false;
+    // a bucket's count becomes the number of entries in the buckets above it; lane t has the buckets
+    // kBuckets - 1 - t kOf downwards
+    int own[kOf], sum = 0;
+#pragma unroll
+    for (int i = 0; i < kOf; ++i) {
+        own[i] = counts[kBuckets - 1 - (threadIdx.x * kOf + i)];
+        sum += own[i];
+    }
+    int upto = sum;
+    for (int step = 1; step < 64; step *= 2) {
+        const int other = __shfl_up(upto, step);
+        if ((int)(threadIdx.x & 63) >= step)
+            upto += other;
+    }
+    if ((threadIdx.x & 63) == 63)
+        sh.tally[0][threadIdx.x >> 6] = upto;
+    __syncthreads();
+    int above = upto - sum;
+    for (int w = 0; w < (int)threadIdx.x >> 6; ++w)
+        above += sh.tally[0][w];
+#pragma unroll
+    for (int i = 0; i < kOf; ++i) {
+        counts[kBuckets - 1 - (threadIdx.x * kOf + i)] = above;
+        above += own[i];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i])
+            list[counts[((uint32_t)(mine[i] >> 32) - low) >> shift] + place[i]] = mine[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kEach; ++i)
+        if (mine[i]) {
+            const int bucket = ((uint32_t)(mine[i] >> 32) - low) >> shift;
+            const int first = counts[bucket], end = bucket ? counts[bucket - 1] : have;
+            int rank = first;
+            for (int at = first; at < end; ++at)
+                rank += list[at] > mine[i];
+            put(rank, mine[i]);
+        }
+    return true;
+}
+
 // Writes the k best of the list (at least k entries) in order.  The list has been written before a
-// barrier and has room for two entries more.
-template <typename E, int T>
-__device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have)
+// barrier and has room for two entries more; `counts` holds CAP >= 1024 integers.
+template <typename E, int T, int CAP>
+__device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have, int *counts, Shared<T> &sh)
 {
     typedef typename E::item item;
     const item *in = reinterpret_cast<const item *>(a.in + row * a.stride);
@@ -274,6 +378,10 @@ __device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have
         const float value = value_of(entry);
         values[rank] = value == 0.0f || value != value ? in[index] : E::put(value);
         indices[rank] = (int32_t)index;
+    };
+    auto put_best = [&](int rank, uint64_t entry) {
+        if (rank < a.k)
+            put(rank, entry);
     };
     if (have <= 256) {
         // a lane per entry counts what exceeds it: have / 2 reads of LDS, the same address in all lanes
@@ -287,11 +395,12 @@ __device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have
                 const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list + i);
                 rank += (two.x > mine) + (two.y > mine);
             }
-            if (rank < a.k)
-                put(rank, mine);
+            put_best(rank, mine);
         }
         return;
     }
+    if (rank_by_buckets<T, CAP>(list, have, counts, sh, put_best))
+        return;
     int size = 512;
     while (size < have)
         size *= 2;
@@ -382,17 +491,21 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
     // -- what reaches it
     const uint64_t bound = (uint64_t)key << 32;
     const int64_t group = (int64_t)kChunk << shift;
-    const int vectors = kAhead << shift;         // of a group
+    const int groups = (int)((n + group - 1) / group) * T, vectors = kAhead << shift;       // of a group
     collect<E, T, CAP>(
-        in, n, bound, top, a.k, list, again, sh, turn, (int)((n + group - 1) / group) * T, vectors,
-        [&](int g) { return maxima[g]; },
+        in, n, bound, top, a.k, list, again, sh, turn, groups, vectors,
+        [&](uint32_t key) {
+            for (int g = threadIdx.x; g < groups; g += T)
+                if (maxima[g] >= key)
+                    list_group<T, CAP>(g, again, sh);
+        },
         [&](int g, int v) { return (g / T) * group + (v * T + g % T) * (int64_t)kItems; });
     if (LSE) {
         stats = nbh_softmax_group<T>(stats, a.scale, sh.stats);
         if (threadIdx.x == 0)
             a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
-    write_ranked<E, T>(a, row, list, sh.count);
+    write_ranked<E, T, CAP>(a, row, list, sh.count, again, sh);
 }
 
 // The largest of each eight lanes, in all eight.
@@ -486,13 +599,19 @@ template <typename E, bool LSE, int T, int P, int CAP> __global__ __launch_bound
     }
     const uint64_t bound = (uint64_t)bound_of<T>(peaks, a.k, sh, turn, top) << 32;
     collect<E, T, CAP>(
-        in, a.vocab, bound, top, a.k, list, again, sh, turn, groups, 8 * a.pieces, [&](int g) { return maxima[g]; },
+        in, a.vocab, bound, top, a.k, list, again, sh, turn, groups, 8 * a.pieces,
+        [&](uint32_t key) {
+#pragma unroll
+            for (int g = 0; g < P; ++g)
+                if (peaks[g] && peaks[g] >= key)
+                    list_group<T, CAP>(g * T + threadIdx.x, again, sh);
+        },
         [&](int g, int v) {
             const int64_t piece = (int64_t)(g / 64) * a.pieces + v / 8;
             const int lane = g % 64 / 8 * 8 + v % 8, j = g % 8;
             return piece * kPiece - before + (j * 64 + lane) * kItems;
         });
-    write_ranked<E, T>(a, row, list, sh.count);
+    write_ranked<E, T, CAP>(a, row, list, sh.count, again, sh);
 }
 
 // Workgroups of the first launch per row and their pieces; 0 tiles: one launch.  `spare`: entries before a
@@ -531,9 +650,9 @@ template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t 
             if (a.tiles * 64 > 4096)
                 top_finish<E, LSE, 512, kMostGroups / 512, 4096><<<grid, dim3(512), 0, stream>>>(a);
             else if (a.k > 128)
-                top_finish<E, LSE, 512, 8, 4096><<<grid, dim3(512), 0, stream>>>(a);
+                top_finish<E, LSE, 1024, 4, 4096><<<grid, dim3(1024), 0, stream>>>(a);
             else
-                top_finish<E, LSE, 256, 16, 1024><<<grid, dim3(256), 0, stream>>>(a);
+                top_finish<E, LSE, 512, 8, 1024><<<grid, dim3(512), 0, stream>>>(a);
         }
         if (const int status = nbh_launch_status())
             return status;
