@@ -361,7 +361,7 @@ enum nbh_row_dtype { NBH_ROW_F32 = 0, NBH_ROW_F16 = 1, NBH_ROW_BF16 = 2 };
  * in float32, rounded once.  Tokens outside [0, vocab) are skipped, offsets are clamped
  * to the arrays.  `repetition`, `presence`, `frequency`: one float32 per row, or NULL for
  * the value beside them.  `out` is of the logits' type or float32 and may be the logits
- * themselves.  Fewer than 2^30 tokens and 2^31 pairs. */
+ * themselves.  Fewer than 2^30 tokens and as many pairs. */
 struct nbh_logits_adjust_args {
     int64_t struct_bytes;              /* sizeof(struct nbh_logits_adjust_args) */
     const void *logits;

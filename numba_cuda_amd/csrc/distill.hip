@@ -448,10 +448,17 @@ template <typename E> __global__ __launch_bounds__(256) void distill_named(Disti
 }
 
 // How a call is spread.
-//   kRows    one workgroup per row does everything
-//   kParts   launches of small workgroups for the statistics, then a wavefront per row for the loss alone, or
-//            with the gradient `splits` workgroups per row, four per compute unit, for stretches of `slice`
-//   kFlat    the gradient by itself in three launches, where the rows hold 64 MiB or more
+//   kRows     one workgroup per row does everything; for the gradient by itself `splits` of them, each a
+//             stretch of `slice` entries
+//   kInParts  a launch of small workgroups for the statistics, then a wavefront per row for the loss alone, or
+//             with the gradient `splits` workgroups per row, four per compute unit
+//   kFlat     the gradient by itself in three launches
+// Measured, one launch against the two of kInParts for the loss, k = 32, bfloat16: 4 x 32768 14 and 18 us,
+// 256 x 131072 19 and 20, 4096 x 32768 53 and 52, 1024 x 131072 53 and 50; float32: 4 x 131072 20 and 17,
+// 256 x 131072 28 and 29, 4096 x 32768 96 and 90.  For both, bfloat16: 4 x 32768 16 and 20, 4 x 131072 22 and
+// 20, 64 x 131072 23 and 22, 256 x 131072 35 and 47; float32: 4 x 131072 25 and 20, 64 x 131072 28 and 27.  One
+// launch against the three of kFlat, float32: 256 x 32768 16 and 24, 256 x 131072 52 and 51, 1024 x 100003 193
+// and 157.
 enum Way { kRows, kInParts, kFlat };
 struct Spread {
     Way way;
@@ -462,21 +469,23 @@ struct Spread {
 Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what, int spare)
 {
     const int64_t items = dtype == NBH_ROW_F32 ? 4 : 8;
-    const int64_t chunk = kStatsThreads * kNbhAhead * items, tile = kStatsThreads * kStatsVecs * items;
+    const int64_t chunk = 256 * kNbhAhead * items;           // 16 KiB, a step of the row kernel
+    const int64_t tile = kStatsThreads * kStatsVecs * items;
     const int64_t flat = kFlatThreads * kFlatVecs * items;
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
-    if (what == kGrad && rows * vocab >= ((int64_t)64 << 20) / 16 * items)
-        return {kFlat,
-                (int)((vocab + spare + flat - 1) / flat), 1, vocab};
+    const bool large = rows * vocab >= ((int64_t)128 << 20) / 16 * items;
     const int tiles = (int)((vocab + spare + tile - 1) / tile);
+    if (what == kGrad && large)
+        return {kFlat, (int)((vocab + spare + flat - 1) / flat), 1, vocab};
     if (what == kLoss)
-        return {chunks > 1 ? kInParts : kRows, tiles, 1, vocab};
+        return {large || (rows < 256 && vocab > 24 * chunk) ? kInParts : kRows, tiles, 1, vocab};
+    if (what == (kLoss | kGrad) && (rows >= 128 || vocab <= 12 * chunk))
+        return {kRows, tiles, 1, vocab};
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
         splits = chunks;
     const int64_t each = (chunks + splits - 1) / splits;
-    splits = (chunks + each - 1) / each;
-    return {what != kGrad && splits > 1 ? kInParts : kRows, tiles, (int)splits, each * chunk};
+    return {what == kGrad ? kRows : kInParts, tiles, (int)((chunks + each - 1) / each), each * chunk};
 }
 
 template <typename E>

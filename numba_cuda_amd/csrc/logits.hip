@@ -245,7 +245,7 @@ extern "C" int nbh_logits_adjust(const struct nbh_logits_adjust_args *p, nbh_str
         return 0;
     const bool same = p->out_dtype == p->dtype;
     if (!p->logits || !p->out || p->dtype < 0 || p->dtype > NBH_ROW_BF16 || !(same || p->out_dtype == NBH_ROW_F32) ||
-        p->vocab > INT32_MAX || p->n_tokens < 0 || p->n_tokens >= (1 << 30) || p->n_bias < 0 || p->n_bias > INT32_MAX)
+        p->vocab > INT32_MAX || p->n_tokens < 0 || p->n_tokens >= (1 << 30) || p->n_bias < 0 || p->n_bias >= (1 << 30))
         return (int)hipErrorInvalidValue;
     auto width = [](int64_t b) { return b == 4 || b == 8; };
     const bool history = p->tokens && p->n_tokens, biases = p->bias_tokens && p->n_bias;

@@ -505,7 +505,7 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
         if (threadIdx.x == 0)
             a.lse[row] = nbh_softmax_lse(stats, a.temperature, a.scale);
     }
-    write_ranked<E, T, CAP>(a, row, list, sh.count, again, sh);
+    write_ranked<E, T, CAP>(a, row, list, sh.count < CAP ? sh.count : CAP, again, sh);
 }
 
 // The largest of each eight lanes, in all eight.
@@ -611,7 +611,7 @@ template <typename E, bool LSE, int T, int P, int CAP> __global__ __launch_bound
             const int lane = g % 64 / 8 * 8 + v % 8, j = g % 8;
             return piece * kPiece - before + (j * 64 + lane) * kItems;
         });
-    write_ranked<E, T, CAP>(a, row, list, sh.count, again, sh);
+    write_ranked<E, T, CAP>(a, row, list, sh.count < CAP ? sh.count : CAP, again, sh);
 }
 
 // Workgroups of the first launch per row and their pieces; 0 tiles: one launch.  `spare`: entries before a
@@ -625,10 +625,11 @@ struct Spread {
 Spread spread_of(int64_t rows, int64_t vocab, int dtype, int spare)
 {
     const int64_t piece = 64 * kPieceVecs * (dtype == NBH_ROW_F32 ? 4 : 8);
-    const int64_t all = (vocab + spare + piece - 1) / piece;
+    // (the number of pieces per workgroup does not depend on `spare`: a workspace for the largest serves all)
+    const int64_t all = (vocab + spare + piece - 1) / piece, most = (vocab + 7 + piece - 1) / piece;
     if (rows >= 128 || vocab <= 20 * piece)
         return {0, 0};
-    const int64_t pieces = (all + kMostGroups / 64 - 1) / (kMostGroups / 64);
+    const int64_t pieces = (most + kMostGroups / 64 - 1) / (kMostGroups / 64);
     return {(int)((all + pieces - 1) / pieces), (int)pieces};
 }
 

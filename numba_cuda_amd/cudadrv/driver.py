@@ -758,6 +758,7 @@ class Context:
         self._scratch = {}          # stream handle -> (address, bytes, memory) of nbh_reduce's scratch
         self._scratch_tls = threading.local()   # the same for each thread's per-thread default stream
         self._workspaces = {}       # stream handle -> (address, bytes, memory) for the row operators
+        self.workspace_lock = threading.Lock()
         self._result_cells = _ResultCells()
 
     @property
@@ -911,8 +912,10 @@ class Context:
     def workspace(self, stream_handle, nbytes):
         """(address, size, memory) of at least `nbytes` bytes for the row operators on the given
         stream (kernels/logits.py), kept and grown as calls need it.  Whoever launches work
-        that uses it holds on to the memory until the launch is made: another thread may
-        replace the entry meanwhile.  Kept per thread for the per-thread default stream."""
+        that uses it holds on to the memory until the launches are made (another thread may
+        replace the entry meanwhile) and makes them under `workspace_lock`, so that the launches
+        of two threads' calls on one stream do not mix.  Kept per thread for the per-thread
+        default stream."""
         if stream_handle == HIP_STREAM_PER_THREAD:
             entry = getattr(self._scratch_tls, "workspace", None)
             if entry is None or entry[1] < nbytes:

@@ -274,6 +274,16 @@ def _workspace(given, nbytes, handle):
 _NO_WORKSPACE = (0, 0, None)
 
 
+def _launch(space, entry, *args):
+    """A call that may be several launches.  Those of two threads that share a stream's workspace must not
+    come between each other: the second would write what the first has still to read."""
+    if space is _NO_WORKSPACE:
+        entry(*args)
+    else:
+        with devices.get_context().workspace_lock:
+            entry(*args)
+
+
 # ---- penalties, biases, masks --------------------------------------------------------------
 
 def _per_row(value, name, rows, stream, number, keep):
@@ -432,8 +442,8 @@ def top(logits, k, *, values=None, indices=None, lse=None, temperature=1.0, work
     _refuse_overlaps(results, [(address, rows, vocab * _SIZE[code], stride, "logits")])
     if rows:
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_top_workspace(rows, vocab, k, code), handle)
-        _driver.driver.nbh_rows_top(address, rows, vocab, stride, code, k, v[0], v[3], i[0], i[3], lse_address,
-                                    temperature, space[0] or None, space[1], handle or None)
+        _launch(space, _driver.driver.nbh_rows_top, address, rows, vocab, stride, code, k, v[0], v[3], i[0], i[3],
+                lse_address, temperature, space[0] or None, space[1], handle or None)
     return (values, indices, lse) if wanted else (values, indices)
 
 
@@ -492,10 +502,10 @@ def _distill(what, grad_loss, student, values, indices, temperature, teacher_lse
 
     if rows:
         space = _workspace(workspace, _driver.driver.lib.nbh_rows_distill_workspace(rows, vocab, k, code, what), handle)
-        _driver.driver.nbh_rows_distill(
-            _DISTILL.pack(_DISTILL_SIZE, what, address, rows, vocab, stride, code, v[0], i[0], k, v[3], v[4], i[3], i[4],
-                          teacher_address, grad_address, grad_stride, grad_value, temperature, loss_address,
-                          lse_address, out_address, out_stride, space[0], space[1]), handle or None)
+        arguments = _DISTILL.pack(_DISTILL_SIZE, what, address, rows, vocab, stride, code, v[0], i[0], k, v[3], v[4], i[3],
+                                  i[4], teacher_address, grad_address, grad_stride, grad_value, temperature,
+                                  loss_address, lse_address, out_address, out_stride, space[0], space[1])
+        _launch(space, _driver.driver.nbh_rows_distill, arguments, handle or None)
     return loss, lse, out
 
 

@@ -362,11 +362,63 @@ def test_no_rows(call):
 @pytest.mark.parametrize("name", cases.DTYPES)
 @pytest.mark.parametrize("in_place, repeated", [(False, False), (True, True)])
 def test_large_gradient_by_itself(name, in_place, repeated):
-    rows, vocab = (700, 26003) if name == "float32" else (1300, 27001)      # over 64 MiB: three launches
+    rows, vocab = (1300, 27001) if name == "float32" else (2500, 27001)      # over 128 MiB: three launches
     assert logits.distill_workspace(rows, vocab, 20, cases.np_dtype(name), loss=False, grad=True) > 0
     cases.check_distill(cuda, rows, vocab, name, 20, what="apart", in_place=in_place, repeated=repeated,
                         pad=0 if in_place else 5, full=not repeated)
 
 
 def test_large_gradient_of_special_rows():
-    cases.check_distill(cuda, 900, 20011, "float32", 6, what="apart", kind="edge", temperature=0.7)
+    cases.check_distill(cuda, 1700, 20011, "float32", 6, what="apart", kind="edge", temperature=0.7)
+
+
+def test_two_threads_on_one_stream():
+    """Calls of several launches that share the stream's workspace, from two host threads."""
+    import threading
+    rng = np.random.default_rng(12)
+    stream = cuda.stream()
+    hosts = [rng.standard_normal((2, 100003)).astype(np.float32) for _ in range(2)]
+    arrays = [cuda.to_device(h) for h in hosts]
+    results, errors = [[], []], []
+
+    def work(n):
+        try:
+            cuda.current_context()
+            for _ in range(50):
+                v, i, z = logits.top(arrays[n], 7, lse=True, stream=stream)
+                results[n].append((i, z, logits.distill_loss(arrays[n], v, i, stream=stream)[0]))
+        except Exception as error:      # noqa: BLE001
+            errors.append(error)
+    threads = [threading.Thread(target=work, args=(n,)) for n in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    stream.synchronize()
+    for n, host in enumerate(hosts):
+        want = logits64.top(host, 7)
+        first = None
+        for i, z, loss in results[n]:
+            got = (i.copy_to_host(), z.copy_to_host(), loss.copy_to_host())
+            stream.synchronize()
+            assert np.array_equal(got[0], want)
+            first = first or got
+            assert np.array_equal(got[1], first[1]) and np.array_equal(got[2], first[2])
+
+
+@pytest.mark.parametrize("name, vocab", [("float32", 524288), ("float32", 524289), ("bfloat16", 1048576), ("float16", 1500001)])
+def test_very_long_rows(name, vocab):
+    """At and past the number of entries from which a workgroup of top's first launch takes several pieces."""
+    rng = np.random.default_rng(vocab)
+    a, x = cases.rows_like(rng, 2, vocab, name)
+    d = cuda.to_device(a)
+    for k in (1, 1000):
+        v, i, z = logits.top(d, k, lse=True)
+        want = np.argsort(-x, axis=1, kind="stable")[:, :k]
+        assert np.array_equal(i.copy_to_host(), want)
+        assert np.abs(z.copy_to_host() - logits64.lse(x)).max() < 1e-5 * 30
+    loss, lse, grad = logits.distill_loss_and_grad(1.0, d, v, i)
+    wl, wz, wg = logits64.distill(x, cases.decode(v.copy_to_host()), want, 1.0, None, [1.0, 1.0])
+    assert np.abs(loss.copy_to_host() - wl).max() < 1e-4 and np.abs(lse.copy_to_host() - wz).max() < 3e-4
+    cases.close(cases.decode(grad.copy_to_host()), wg, cases.HALF_STEP[name] * np.abs(wg) + 1e-4 * np.abs(wg) + 1e-6, "gradient")

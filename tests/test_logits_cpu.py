@@ -251,4 +251,4 @@ def test_the_entry_points_check_their_arguments():
     assert lib.nbh_rows_distill(logits._DISTILL.pack(8, *([0] * 24)), None) != 0
     # long rows are spread over workgroups, short ones are not
     assert lib.nbh_rows_top_workspace(1, 131072, 50, 0) > 0 == lib.nbh_rows_top_workspace(4096, 1000, 50, 0)
-    assert lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 1) > 0 == lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 2)
+    assert lib.nbh_rows_distill_workspace(1, 1310720, 8, 2, 1) > 0 == lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 2)
