@@ -9,8 +9,13 @@
 // the end of the first in the caches, writes the gradient as a * 2^((s - m) * c) for every entry, and behind
 // a barrier the few entries the teacher names are written again with their p_j taken off.  The loss
 // alone, and few rows, are spread: small workgroups in the order of memory for the statistics, then a launch
-// that joins them and does the rest.  A large gradient by itself is a copy with arithmetic: a launch prepares two numbers
-// for each row, small workgroups in memory order do the copy, a last launch writes the named entries.
+// that joins them and does the rest.  A large gradient by itself is a copy with arithmetic: a launch prepares two
+// numbers for each row, small workgroups in memory order do the copy, a last launch writes the named entries.
+//
+// Bound by memory: the loss reads a row once (2048 x 50021 float16: 36 + 6 us, 205 MB at 5.8 TB/s in the first
+// launch), the gradient reads and writes it (1024 x 100003 float32: 10 + 139 + 5 us, 819 MB at 5.9 TB/s in the
+// second).  Both at once read it from memory once (4096 x 131072 bfloat16: 2.15 GB, 423 us, 5.1 TB/s); beside the
+// traffic there are two exponentials per entry, some 0.28 ms of the vector units' time.
 #include "rows.h"
 
 namespace {
@@ -51,6 +56,7 @@ struct Distill {
 };
 
 // The statistics of 8 KiB of a row per workgroup, in the order of memory, one pair of numbers per wavefront.
+// 2048 x 50021 float16: 35.8 us; 4 KiB per wavefront 39.4, 16 KiB 40.7, two wavefronts 39.6, four 45.
 template <typename E>
 __global__ __launch_bounds__(kStatsThreads) void distill_stats(Distill a)
 {
@@ -70,12 +76,7 @@ __global__ __launch_bounds__(kStatsThreads) void distill_stats(Distill a)
             raw[j] = nbh_row_load_raw<E, true>(in, first + (j * T + (int)threadIdx.x) * kItems, a.vocab, E::lowest);
     }
     nbh_softmax stats = nbh_softmax_empty();
-#pragma unroll
-    for (int j = 0; j < kStatsVecs; ++j) {
-        float f[kItems];
-        E::unpack(raw[j], f);
-        nbh_softmax_add(stats, f, nbh_row_most(f), a.scale);
-    }
+    nbh_row_stats<E>(stats, raw, a.scale);
     stats = nbh_softmax_wave(stats, a.scale);
     if ((threadIdx.x & 63) == 0)
         a.parts[(at * a.tiles + tile) * (T / 64) + threadIdx.x / 64] = stats;
@@ -288,14 +289,28 @@ __device__ __forceinline__ Named named_of(const Distill &a, const Teacher &t, in
     return {index, whole * nbh_softmax_term(t.student[j], s.peak, a.scale) - factor * own};
 }
 
-template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void distill_rows(Distill a)
+// With 512 lanes the loss and the gradient together keep the beginning of the row, 96 KiB of it in registers and
+// 64 KiB in LDS, so that only what lies behind is read again, from the caches.  Two such workgroups fill a compute
+// unit.  4096 x 131072 bfloat16: nothing kept 460 us (2.07 GB of reads leave the L2 caches instead of 1.07), 32 KiB
+// in LDS 446, 64 KiB 442, and in registers 32 KiB 435, 64 KiB 430, 96 KiB 423; one workgroup per compute unit with
+// 128 KiB in LDS 473.
+template <int T, int WHAT> struct Kept {
+    static constexpr bool some = T == 512 && WHAT == (kLoss | kGrad);
+    static constexpr int held = some ? 3 : 0, stored = some ? 2 : 0, waves = some ? 4 : 1;
+};
+template <typename E, int T, int WHAT>
+__global__ __launch_bounds__(T, (Kept<T, WHAT>::waves)) void distill_rows(Distill a)
 {
     typedef typename E::item item;
+    typedef Kept<T, WHAT> Keep;
     constexpr int kItems = E::items;
+    constexpr int64_t kChunk = kNbhAhead * T * kItems;
     extern __shared__ char lds[];
     __shared__ nbh_softmax room[T / 64];
     __shared__ float mass;
     __shared__ int some, repeated;
+    __shared__ nbh_u32x4 store[Keep::some ? Keep::stored * kNbhAhead * T : 1];
+    nbh_u32x4 hold[Keep::some ? Keep::held * kNbhAhead : 1];
     Teacher teacher;
     teacher.place(lds, a.k);
 
@@ -305,6 +320,10 @@ template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void dist
     const int split = kWhole ? 0 : blockIdx.x % a.splits;
     const item *in = reinterpret_cast<const item *>(a.student + row * a.stride);
     const int64_t begin = split * a.slice, end = a.vocab < begin + a.slice ? a.vocab : begin + a.slice;
+    // entries 0 .. held are in `hold`, held .. kept in `store`
+    const int64_t held = a.vocab >= Keep::held * kChunk ? Keep::held * kChunk : 0;
+    const int64_t chunks = (a.vocab - held) / kChunk;
+    const int64_t kept = held + (chunks < Keep::stored ? chunks : Keep::stored) * kChunk;
 
     if (threadIdx.x < 64) {
         load_teacher<E, WHAT>(a, row, WHAT & kLoss ? 0 : begin, WHAT & kLoss ? a.vocab : end, teacher);
@@ -321,7 +340,29 @@ template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void dist
             stats = joined_stats(a, row - a.row0);
             __syncthreads();
         } else {
-            stats = nbh_softmax_group<T>(nbh_row_stats<E, T, false>(in, 0, a.vocab, a.scale), a.scale, room);
+            stats = nbh_softmax_empty();
+            if (Keep::some && held) {
+#pragma unroll
+                for (int j = 0; j < Keep::held * kNbhAhead; ++j)
+                    hold[j] = E::template load<false>(in + (j * T + threadIdx.x) * kItems);
+                // (not through a reference to `hold`: that leaves it in scratch memory)
+#pragma unroll
+                for (int j = 0; j < Keep::held * kNbhAhead; ++j) {
+                    float f[kItems];
+                    E::unpack(hold[j], f);
+                    nbh_softmax_add(stats, f, nbh_row_most(f), a.scale);
+                }
+            }
+            nbh_row_stream<E, T, false>(
+                in, held, a.vocab, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
+                    if (at < kept) {
+#pragma unroll
+                        for (int j = 0; j < kNbhAhead; ++j)
+                            store[((at - held) / kChunk * kNbhAhead + j) * T + threadIdx.x] = raw[j];
+                    }
+                    nbh_row_stats<E>(stats, raw, a.scale);
+                });
+            stats = nbh_softmax_group<T>(stats, a.scale, room);
         }
         student = student_of(stats);
         if (a.lse && split == 0 && threadIdx.x == 0)
@@ -348,23 +389,43 @@ template <typename E, int T, int WHAT> __global__ __launch_bounds__(T) void dist
     }
     const float whole = factor * mass * student.base, product = student.peak * a.scale;
     const bool near = nbh_softmax_near(product);
-    nbh_row_stream<E, T, true, true>(
-        in, begin, end, [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
+    auto write = [&](int64_t at, const nbh_u32x4(&raw)[kNbhAhead]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 0; j < kNbhAhead; ++j) {
-                float f[kItems];
-                E::unpack(raw[j], f);
-                if (near) {
+        for (int j = 0; j < kNbhAhead; ++j) {
+            float f[kItems];
+            E::unpack(raw[j], f);
+            if (near) {
 #pragma unroll
-                    for (int i = 0; i < kItems; ++i)
-                        f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
-                } else {
-                    for (int i = 0; i < kItems; ++i)
-                        f[i] = whole * nbh_exp2((f[i] - student.peak) * a.scale);
-                }
-                nbh_row_store<E, true>(out, at + (j * T + threadIdx.x) * kItems, end, f);
+                for (int i = 0; i < kItems; ++i)
+                    f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
+            } else {
+                for (int i = 0; i < kItems; ++i)
+                    f[i] = whole * nbh_exp2((f[i] - student.peak) * a.scale);
             }
-        });
+            nbh_row_store<E, true>(out, at + (j * T + threadIdx.x) * kItems, end, f);
+        }
+    };
+    nbh_row_stream<E, T, true, true>(in, begin + kept, end, write);
+    if (Keep::some) {
+        for (int64_t at = kept; at > held;) {
+            at -= kChunk;
+            nbh_u32x4 raw[kNbhAhead];
+#pragma unroll
+            for (int j = 0; j < kNbhAhead; ++j)
+                raw[j] = store[((at - held) / kChunk * kNbhAhead + j) * T + threadIdx.x];
+            write(at, raw);
+        }
+        if (held) {
+#pragma unroll
+            for (int chunk = 0; chunk < Keep::held; ++chunk) {
+                nbh_u32x4 raw[kNbhAhead];
+#pragma unroll
+                for (int j = 0; j < kNbhAhead; ++j)
+                    raw[j] = hold[chunk * kNbhAhead + j];
+                write(chunk * kChunk, raw);
+            }
+        }
+    }
     __syncthreads();
     teacher.repeated = repeated;
     for (int j = threadIdx.x; j < a.k; j += T)
@@ -392,7 +453,8 @@ template <typename E> __global__ __launch_bounds__(64) void distill_plan(Distill
     for (int j = threadIdx.x; j < a.k; j += 64)
         a.named[(row - a.row0) * a.k + j] = zero ? Named{-1, 0.0f} : named_of(a, teacher, j, student, whole, factor);
 }
-// Second: small workgroups in the order of memory.
+// Second: small workgroups in the order of memory, a vector per lane (1024 x 100003 float32: 139 us; with two
+// vectors 161, with four 149, four wavefronts 140).
 constexpr int kFlatThreads = 64, kFlatVecs = 1;
 template <typename E> __global__ __launch_bounds__(kFlatThreads) void distill_flat(Distill a)
 {
@@ -459,10 +521,18 @@ template <typename E> __global__ __launch_bounds__(256) void distill_named(Disti
 // 20, 64 x 131072 23 and 22, 256 x 131072 35 and 47; float32: 4 x 131072 25 and 20, 64 x 131072 28 and 27.  One
 // launch against the three of kFlat, float32: 256 x 32768 16 and 24, 256 x 131072 52 and 51, 1024 x 100003 193
 // and 157.
+// Rows of up to 16 KiB, a chunk of the row kernel, are always kRows with a wavefront each: what a workgroup does
+// once per row takes longer than the row, and this way most of the rows of a call are under way together.
+// bfloat16, 64, 256 and 512 lanes: loss 4096 x 1024 13, 22 and 40 us, 4096 x 8192 20, 22 and 43, 4096 x 16384 35,
+// 35 and 36; gradient 4096 x 1024 16, 30 and 53, 4096 x 8192 33, 34 and 53; both 4096 x 1024 19, 42 and 78, 4096 x
+// 8192 40, 40 and 74.  In several launches: loss 131072 x 1024 280 instead of 171, 16384 x 8192 70 instead of 59,
+// gradient 288 instead of 234 and 153 instead of 137.
+// Both at once, 256 and 512 lanes: 4096 x 16384 67 and 97, 4096 x 32768 125 and 130, 512 x 16384 17 and 17, 256 x
+// 32768 18 and 17, 4096 x 50021 242 and 224, 4096 x 65536 244 and 209.
 enum Way { kRows, kInParts, kFlat };
 struct Spread {
     Way way;
-    int tiles, splits;
+    int tiles, lanes, splits;            // lanes of the row kernel
     int64_t slice;
 };
 // `spare`: entries before a row's beginning that its first vector may hold
@@ -473,23 +543,24 @@ Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what, int spare)
     const int64_t tile = kStatsThreads * kStatsVecs * items;
     const int64_t flat = kFlatThreads * kFlatVecs * items;
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
-    const bool large = rows * vocab >= ((int64_t)128 << 20) / 16 * items;
+    const bool small = chunks == 1, large = !small && rows * vocab >= ((int64_t)128 << 20) / 16 * items;
     const int tiles = (int)((vocab + spare + tile - 1) / tile);
     if (what == kGrad && large)
-        return {kFlat, (int)((vocab + spare + flat - 1) / flat), 1, vocab};
+        return {kFlat, (int)((vocab + spare + flat - 1) / flat), 0, 1, vocab};
     if (what == kLoss)
-        return {large || (rows < 256 && vocab > 24 * chunk) ? kInParts : kRows, tiles, 1, vocab};
-    if (what == (kLoss | kGrad) && (rows >= 128 || vocab <= 12 * chunk))
-        return {kRows, tiles, 1, vocab};
+        return {large || (rows < 256 && chunks > 24) ? kInParts : kRows, tiles, small ? 64 : 256, 1, vocab};
+    if (what == (kLoss | kGrad) && (rows >= 128 || chunks <= 12))
+        return {kRows, tiles, small ? 64 : chunks <= 4 && rows > 512 ? 256 : 512, 1, vocab};
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
         splits = chunks;
     const int64_t each = (chunks + splits - 1) / splits;
-    return {what == kGrad ? kRows : kInParts, tiles, (int)((chunks + each - 1) / each), each * chunk};
+    return {what == kGrad ? kRows : kInParts, tiles, small ? 64 : 256, (int)((chunks + each - 1) / each),
+            each * chunk};
 }
 
 template <typename E>
-int launch_distill(Distill a, Way way, int64_t rows, int what, hipStream_t stream)
+int launch_distill(Distill a, Way way, int lanes, int64_t rows, int what, hipStream_t stream)
 {
     const size_t bytes = Teacher::bytes(a.k);
     const int64_t most = NBH_ROW_MOST_GROUPS / (way == kRows ? a.splits : a.tiles);
@@ -508,12 +579,22 @@ int launch_distill(Distill a, Way way, int64_t rows, int what, hipStream_t strea
             else
                 distill_rows<E, 256, kLoss | kGrad | kParts><<<split, dim3(256), bytes, stream>>>(a);
         } else if (what == kGrad) {
-            distill_rows<E, 256, kGrad><<<split, dim3(256), bytes, stream>>>(a);
+            if (lanes == 64)
+                distill_rows<E, 64, kGrad><<<split, dim3(64), bytes, stream>>>(a);
+            else
+                distill_rows<E, 256, kGrad><<<split, dim3(256), bytes, stream>>>(a);
         } else if (what == kLoss) {
-            distill_rows<E, 256, kLoss><<<each, dim3(256), bytes, stream>>>(a);
+            if (lanes == 64)
+                distill_rows<E, 64, kLoss><<<each, dim3(64), bytes, stream>>>(a);
+            else
+                distill_rows<E, 256, kLoss><<<each, dim3(256), bytes, stream>>>(a);
         } else {
-            // fewer rows at a time, so that they are still in the caches when they are read again
-            distill_rows<E, 512, kLoss | kGrad><<<each, dim3(512), bytes, stream>>>(a);
+            if (lanes == 64)
+                distill_rows<E, 64, kLoss | kGrad><<<each, dim3(64), bytes, stream>>>(a);
+            else if (lanes == 256)
+                distill_rows<E, 256, kLoss | kGrad><<<each, dim3(256), bytes, stream>>>(a);
+            else
+                distill_rows<E, 512, kLoss | kGrad><<<each, dim3(512), bytes, stream>>>(a);
         }
         if (const int status = nbh_launch_status())
             return status;
@@ -590,10 +671,10 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     nbh_stream_report report(s);
     switch (p->dtype) {
     case NBH_ROW_F32:
-        return launch_distill<nbh_row_f32>(a, spread.way, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f32>(a, spread.way, spread.lanes, p->rows, (int)p->what, s);
     case NBH_ROW_F16:
-        return launch_distill<nbh_row_f16>(a, spread.way, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_f16>(a, spread.way, spread.lanes, p->rows, (int)p->what, s);
     default:
-        return launch_distill<nbh_row_bf16>(a, spread.way, p->rows, (int)p->what, s);
+        return launch_distill<nbh_row_bf16>(a, spread.way, spread.lanes, p->rows, (int)p->what, s);
     }
 }

@@ -11,6 +11,11 @@
 // a row reads the whole history, from L2.  Bias pairs of the tile go to a short list.  Integer LDS atomics
 // only, and of the pairs the one with the largest number counts: the order in which lanes arrive changes
 // nothing.
+//
+// Bound by memory where rows are many, by the start of a launch and the walk through the history where they are
+// few.  Kernel times: 256 x 131072 bfloat16 to float32 with masks, biases and histories of 4096 38 us, its 208 MB
+// at 5.5 TB/s (72 us while results of four bytes left a lane in two stores 16 bytes apart, hence the half
+// vectors; 98 us with inputs read past the caches); 8 x 131072 float32, histories of 131071 13 us; 1 x 32768 4 us.
 #include "rows.h"
 
 namespace {
@@ -229,8 +234,12 @@ int launch_adjust(Adjust a, int64_t rows, hipStream_t stream)
 template <typename In, typename Out>
 int launch_adjust(const Adjust &a, int64_t rows, hipStream_t stream)
 {
-    // Long histories cost more than the row: fewer, larger workgroups read them less often.
-    if (a.n_tokens / rows > 8192)
+    // Every tile of a row reads the whole history, so long ones are read by fewer, larger workgroups; they start
+    // and end less evenly.  256 x 4096 against 1024 x 8192 on rows of 131072 bfloat16, mean history 8192: 64 rows
+    // 17.4 and 18.9 us, 256 rows 48 and 55; 16384: 64 rows 22.8 and 20.6, 256 rows 62 and 64; 65536: 1 row 34 and
+    // 16, 64 rows 64 and 40, 256 rows 164 and 125.  (8 rows of 131072 float32, 65536: tiles of 16384 18.8 us, of
+    // 8192 16.7, of 32768 21.9.)
+    if (a.n_tokens / rows > 12288)
         return launch_adjust<In, Out, 1024, 8192>(a, rows, stream);
     return launch_adjust<In, Out, 256, 4096>(a, rows, stream);
 }

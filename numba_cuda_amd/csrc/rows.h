@@ -311,20 +311,16 @@ __device__ __forceinline__ void nbh_row_stream(const typename E::item *in, int64
     if (!BACK && rest < end)
         chunk(rest, tail);
 }
-template <typename E, int T, bool NT>
-__device__ __forceinline__ nbh_softmax nbh_row_stats(const typename E::item *in, int64_t begin, int64_t end, float scale)
+// N vectors of a row's statistics.
+template <typename E, int N>
+__device__ __forceinline__ void nbh_row_stats(nbh_softmax &stats, const nbh_u32x4 (&raw)[N], float scale)
 {
-    nbh_softmax stats = nbh_softmax_empty();
-    nbh_row_stream<E, T, NT>(in, begin, end, [&](int64_t, const nbh_u32x4(&raw)[kNbhAhead])
-                                 __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < kNbhAhead; ++j) {
-            float f[E::items];
-            E::unpack(raw[j], f);
-            nbh_softmax_add(stats, f, nbh_row_most(f), scale);
-        }
-    });
-    return stats;
+    for (int j = 0; j < N; ++j) {
+        float f[E::items];
+        E::unpack(raw[j], f);
+        nbh_softmax_add(stats, f, nbh_row_most(f), scale);
+    }
 }
 
 // Temperatures whose reciprocal is an ordinary float32 number.

@@ -14,6 +14,9 @@
 //     by bisection over all entries, and if it ends on a value that too many share, to the first of them.
 // Short rows: one workgroup does all of that for a row.  Long ones: a first launch of small workgroups in the
 // order of memory finds the groups' maxima and the statistics of the log-sum-exp, a second one does the rest.
+// For many rows one launch is faster, as one row's bisection hides behind another's reading: 4096 x 65536
+// bfloat16, k = 64, 110 us (537 MB at 4.9 TB/s), in two launches 103 + 53.  Few long rows end with the second
+// launch's latency: 16 x 131072 float16, k = 512, 5 + 15 us; 64 x 100003 bfloat16, k = 50, 8 + 10 us.
 #include "rows.h"
 
 namespace {
@@ -640,8 +643,8 @@ template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t 
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
         const dim3 grid((unsigned)now);
         if (a.tiles == 0) {
-            // 256 lanes make 1024 groups, which serve up to k = 256; larger workgroups wait longer at
-            // their barriers (4096 x 65536 bfloat16, k = 64: 124 us, with 512 lanes 140 us)
+            // 256 lanes make up to 2048 groups, which serve up to k = 256; larger workgroups wait longer at
+            // their barriers (4096 x 65536 bfloat16, k = 64: 114 us; a step earlier 124 us, with 512 lanes 140)
             if (a.k <= 256)
                 top_rows<E, LSE, 256, 1024><<<grid, dim3(256), 0, stream>>>(a);
             else

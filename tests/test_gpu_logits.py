@@ -422,3 +422,18 @@ def test_very_long_rows(name, vocab):
     wl, wz, wg = logits64.distill(x, cases.decode(v.copy_to_host()), want, 1.0, None, [1.0, 1.0])
     assert np.abs(loss.copy_to_host() - wl).max() < 1e-4 and np.abs(lse.copy_to_host() - wz).max() < 3e-4
     cases.close(cases.decode(grad.copy_to_host()), wg, cases.HALF_STEP[name] * np.abs(wg) + 1e-4 * np.abs(wg) + 1e-6, "gradient")
+
+
+# rows about the lengths where a row is kept in registers and LDS in other shares, and read by more lanes
+@pytest.mark.parametrize("name, around", [("float32", 4096), ("float32", 24576), ("float32", 32768),
+                                          ("bfloat16", 16384), ("bfloat16", 49152), ("float16", 81920)])
+def test_distill_of_rows_kept_in_part(name, around):
+    for vocab in (around - 1, around, around + 1, around + 100):
+        cases.check_distill(cuda, 3, vocab, name, 40, what="both", pad=5)
+        cases.check_distill(cuda, 3, vocab, name, 1024, what="both", temperature=2.0, in_place=True)
+
+
+@pytest.mark.parametrize("name, vocab", [("float32", 4099), ("float32", 16384), ("bfloat16", 8193), ("float16", 32768)])
+def test_distill_of_many_rows(name, vocab):
+    cases.check_distill(cuda, 520, vocab, name, 20, what="both", in_place=True)
+    cases.check_distill(cuda, 520, vocab, name, 20, what="both", kind="edge", pad=1)
