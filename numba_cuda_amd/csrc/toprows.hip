@@ -278,7 +278,9 @@ __device__ __forceinline__ void collect(const typename E::item *in, int64_t n, u
 
 // Ranks the list's entries by counting them into 1024 buckets of equal width between the smallest and the
 // largest key: put(rank, entry).  False, and nothing done, where a bucket is too crowded to be searched.
-// `counts` holds 1024 integers; the list's order changes.
+// Where the keys are of both signs, the widths are equal in the values: nearly all of the keys between lie about
+// zero (512 of 1024, 4096 rows of bfloat16: 122 us by keys, 60 by values).  `counts` holds 1024 integers; the
+// list's order changes.
 constexpr int kBuckets = 1024, kCrowd = 64;
 template <int T, int CAP, typename F>
 __device__ bool rank_by_buckets(uint64_t *list, int have, int *counts, Shared<T> &sh, F put)
@@ -313,12 +315,24 @@ __device__ bool rank_by_buckets(uint64_t *list, int have, int *counts, Shared<T>
         low = sh.ends[1][w] < low ? sh.ends[1][w] : low;
     }
     const int bits = 32 - __clz((int)(high - low)), shift = bits > 10 ? bits - 10 : 0;
-    int place[kEach];                    // of an entry within its bucket
+    const float least = fmaxf(value_of((uint64_t)low << 32), -1e38f);
+    const float most = fminf(value_of((uint64_t)high << 32), 1e38f);      // NaN: 1e38
+    const bool linear = low < 0x80000000u && high > 0x80000000u && most - least > 1e-30f;
+    const float steep = linear ? kBuckets / (most - least) : 0.0f;
+    auto bucket_of = [&](uint64_t entry) {                   // rises with the entry
+        if (!linear)
+            return (int)(((uint32_t)(entry >> 32) - low) >> shift);
+        const float value = fmaxf(fminf(value_of(entry), most), least);
+        const int bucket = (int)((value - least) * steep);
+        return bucket < kBuckets ? bucket : kBuckets - 1;
+    };
+    int bucket[kEach], place[kEach];     // of an entry, and its place within the bucket
     bool crowded = false;
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         if (mine[i]) {
-            place[i] = atomicAdd(&counts[((uint32_t)(mine[i] >> 32) - low) >> shift], 1);
+            bucket[i] = bucket_of(mine[i]);
+            place[i] = atomicAdd(&counts[bucket[i]], 1);
             crowded |= place[i] >= kCrowd;
         }
     if (__syncthreads_or(crowded))
@@ -352,13 +366,12 @@ __device__ bool rank_by_buckets(uint64_t *list, int have, int *counts, Shared<T>
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         if (mine[i])
-            list[counts[((uint32_t)(mine[i] >> 32) - low) >> shift] + place[i]] = mine[i];
+            list[counts[bucket[i]] + place[i]] = mine[i];
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < kEach; ++i)
         if (mine[i]) {
-            const int bucket = ((uint32_t)(mine[i] >> 32) - low) >> shift;
-            const int first = counts[bucket], end = bucket ? counts[bucket - 1] : have;
+            const int first = counts[bucket[i]], end = bucket[i] ? counts[bucket[i] - 1] : have;
             int rank = first;
             for (int at = first; at < end; ++at)
                 rank += list[at] > mine[i];
@@ -368,7 +381,7 @@ __device__ bool rank_by_buckets(uint64_t *list, int have, int *counts, Shared<T>
 }
 
 // Writes the k best of the list (at least k entries) in order.  The list has been written before a
-// barrier and has room for two entries more; `counts` holds CAP >= 1024 integers.
+// barrier and has room for two entries more; `counts` holds CAP integers, at least 1024 of them if CAP exceeds 256.
 template <typename E, int T, int CAP>
 __device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have, int *counts, Shared<T> &sh)
 {
@@ -386,13 +399,13 @@ __device__ void write_ranked(const Top &a, int64_t row, uint64_t *list, int have
         if (rank < a.k)
             put(rank, entry);
     };
-    if (have <= 256) {
+    if (CAP <= 256 || have <= 256) {
         // a lane per entry counts what exceeds it: have / 2 reads of LDS, the same address in all lanes
         if (threadIdx.x == 0)
             list[have] = 0;
         __syncthreads();
-        if ((int)threadIdx.x < have) {
-            const uint64_t mine = list[threadIdx.x];
+        for (int at = threadIdx.x; at < have; at += T) {
+            const uint64_t mine = list[at];
             int rank = 0;
             for (int i = 0; i < have; i += 2) {
                 const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(list + i);
@@ -460,7 +473,8 @@ template <typename E, bool LSE, int T, int CAP> __global__ __launch_bounds__(T) 
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
         peak[j] = -INFINITY;
-    nbh_row_stream<E, T, false>(in, 0, n, [&](int64_t at, const nbh_u32x4(&raw)[kAhead]) __attribute__((always_inline)) {
+    nbh_row_stream<E, T, false>(in, 0, n, [&](int64_t at, const nbh_u32x4(&raw)[kAhead])
+                                __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < kAhead; ++j) {
             float f[kItems];
@@ -636,16 +650,38 @@ Spread spread_of(int64_t rows, int64_t vocab, int dtype, int spare)
     return {(int)((all + pieces - 1) / pieces), (int)pieces};
 }
 
+// Lanes of the one-launch kernel.  A lane's four vectors give as many maxima for the bound, so T lanes serve well
+// up to k = T; larger workgroups wait longer at their barriers and fewer rows are under way at a time.  A call of
+// one row finishes sooner with more lanes.  Measured, bfloat16:
+//   k <= 64, rows of up to 16 KiB, 64 and 256 lanes: k = 50, 4096 x 1024 21 and 42 us, 4096 x 8192 28 and 35, 2048 x
+//   8192 21 and 22, 1500 x 8192 19 and 17, 64 x 8192 16 and 11; rows of 32 KiB, 4096 of them 44 and 45, of 64 KiB
+//   80 and 65.
+//   k <= 256, 256 and 512 lanes: k = 64, 4096 x 65536 124 and 140; k = 200, 4096 x 1024 118 and 214.
+//   k = 500, 256 and 512 lanes: 512 x 8192 21 and 25, 4096 x 8192 66 and 168; 512 x 32768 34 and 29, 1024 x 32768
+//   44 and 50, 4096 x 32768 118 and 180, 1024 x 50021 57 and 66, 512 x 131072 66 and 51 (k = 300: 2048 x 131072
+//   159 and 143).
+//   k = 1000: 4096 x 1024 117 and 214, 4096 x 8192 222 and 391, 4096 x 32768 799 and 265 (k = 700: 395 and 214).
+int lanes_of(int64_t rows, int64_t vocab, int64_t bytes, int k)
+{
+    const bool brief = vocab * bytes <= (16 << 10);
+    if (brief && k <= 64 && rows >= 2048)
+        return 64;
+    if (brief || k <= 256 || (k <= 512 && rows >= 1024 && vocab * bytes <= (128 << 10)))
+        return 256;
+    return 512;
+}
+
 template <typename E, bool LSE> int launch_top(Top a, int64_t rows, hipStream_t stream)
 {
+    const int lanes = lanes_of(rows, a.vocab, sizeof(typename E::item), a.k);
     const int64_t most = NBH_ROW_MOST_GROUPS / (a.tiles ? a.tiles : 1);
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t now = rows - a.row0 < most ? rows - a.row0 : most;
         const dim3 grid((unsigned)now);
         if (a.tiles == 0) {
-            // 256 lanes make up to 2048 groups, which serve up to k = 256; larger workgroups wait longer at
-            // their barriers (4096 x 65536 bfloat16, k = 64: 114 us; a step earlier 124 us, with 512 lanes 140)
-            if (a.k <= 256)
+            if (lanes == 64)
+                top_rows<E, LSE, 64, 256><<<grid, dim3(64), 0, stream>>>(a);
+            else if (lanes == 256)
                 top_rows<E, LSE, 256, 1024><<<grid, dim3(256), 0, stream>>>(a);
             else
                 top_rows<E, LSE, 512, 4096><<<grid, dim3(512), 0, stream>>>(a);

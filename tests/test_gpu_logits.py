@@ -437,3 +437,27 @@ def test_distill_of_rows_kept_in_part(name, around):
 def test_distill_of_many_rows(name, vocab):
     cases.check_distill(cuda, 520, vocab, name, 20, what="both", in_place=True)
     cases.check_distill(cuda, 520, vocab, name, 20, what="both", kind="edge", pad=1)
+
+
+@pytest.mark.parametrize("name", cases.DTYPES)
+@pytest.mark.parametrize("rows, vocab, k", [(2048, 1009, 64), (2500, 300, 1), (2048, 4096, 33), (2049, 3, 3), (1030, 600, 400),
+                                            (1024, 9000, 300)])
+def test_top_of_many_rows(name, rows, vocab, k):
+    cases.check_top(cuda, rows, vocab, name, k, pad=5)
+    cases.check_top(cuda, rows, vocab, name, k, kind="edge")
+
+
+@pytest.mark.parametrize("k", [1, 10, 64])
+def test_top_of_many_masked_rows(k):
+    rng = np.random.default_rng(19)
+    a = np.full((2100, 4000), np.finfo(np.float32).min, np.float32)
+    a[1::3] = -np.inf
+    a[2::3] = 1.5                                    # all alike
+    for row in range(0, 2100, 7):
+        a[row, rng.integers(0, 4000, row % 300)] = rng.standard_normal(row % 300)
+    a[5] = np.arange(4000)
+    a[6] = -np.arange(4000)
+    values, indices = (o.copy_to_host() for o in logits.top(cuda.to_device(a), k)[:2])
+    order = np.argsort(-a, axis=1, kind="stable")[:, :k]
+    assert np.array_equal(indices, order)
+    assert np.array_equal(values, np.take_along_axis(a, order, 1))
