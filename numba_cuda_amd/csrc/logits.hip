@@ -8,22 +8,21 @@
 //
 // A workgroup owns a tile of one row's vocabulary.  It asks for the tile's logits and mask first and
 // counts the row's history into one LDS word per entry (below) while they are on their way; every tile of
-// a row reads the whole history, from L2.  Bias pairs of the tile go to a short list.  Integer LDS atomics
-// only, and of the pairs the one with the largest number counts: the order in which lanes arrive changes
-// nothing.
+// a row reads the whole history, from L2.  The bias pairs leave the largest of their numbers in the same words
+// afterwards (in words of their own, 256 x 131072 with 64 pairs took 60 us instead of 45, as half as many
+// workgroups fit a compute unit).  Integer LDS atomics only: the order in which lanes arrive changes nothing.
 //
 // Bound by memory where rows are many, by the start of a launch and the walk through the history where they are
-// few.  Kernel times: 256 x 131072 bfloat16 to float32 with masks, biases and histories of 4096 38 us, its 208 MB
-// at 5.5 TB/s (72 us while results of four bytes left a lane in two stores 16 bytes apart, hence the half
-// vectors; 98 us with inputs read past the caches); 8 x 131072 float32, histories of 131071 13 us; 1 x 32768 4 us.
+// few.  256 x 131072 bfloat16 to float32 with masks, 64 biases and histories of 4096 a row: 42 us, its 208 MB at
+// 4.9 TB/s (72 us while results of four bytes left a lane in two stores 16 bytes apart, hence the half vectors; 98
+// us with inputs read past the caches).
 #include "rows.h"
 
 namespace {
 
-// The word of an entry: bit 31 it occurs in the history, bit 30 a pair of the list names it, below them
-// how often it occurs behind the prompt.
-constexpr uint32_t kSeen = 0x80000000u, kBiased = 0x40000000u, kCount = 0x3fffffffu;
-constexpr int kPairs = 256;              // bias pairs a tile lists; the rest of them are looked up in memory
+// The word of an entry: bit 31 it occurs in the history, below it how often it occurs behind the prompt; then
+// again, one more than the number of the last pair that names it.
+constexpr uint32_t kSeen = 0x80000000u, kCount = 0x7fffffffu;
 
 struct Adjust {
     const char *in;
@@ -95,14 +94,12 @@ __device__ __forceinline__ void visit_tokens(const void *p, int bytes, int64_t b
         visit_tokens<T>(static_cast<const int64_t *>(p) + begin, (int)(end - begin), first, n, visit);
 }
 
-template <typename In, typename Out, int T, int TILE>
+template <typename In, typename Out, int T, int TILE, bool BIASES>
 __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
 {
     constexpr int kItems = In::items, kVecs = TILE / (T * kItems);
     static_assert(Out::items == kItems, "as many entries per vector on both sides");
     __shared__ uint32_t words[TILE];
-    __shared__ uint32_t pair_at[kPairs], pair_number[kPairs];
-    __shared__ uint32_t pair_count;
     const int64_t row = a.row0 + blockIdx.x / a.tiles;
     const int tile = blockIdx.x % a.tiles;
     const int64_t first = (int64_t)tile * TILE;
@@ -121,28 +118,28 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
     }
 
     // everything about the row, asked for at once
-    const bool history = a.tokens != nullptr, biases = a.bias_tokens != nullptr;
+    const bool history = a.tokens != nullptr;
     int64_t begin = 0, end = 0, prompt_length = 0, pair0 = 0, pair1 = 0;
     if (history) {
         begin = nbh_row_int(a.offsets, a.offset_bytes, row);
         end = nbh_row_int(a.offsets, a.offset_bytes, row + 1);
         prompt_length = a.prompts ? nbh_row_int(a.prompts, a.prompt_bytes, row) : 0;
     }
-    if (biases) {
+    if (BIASES) {
         pair0 = nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row);
         pair1 = nbh_row_int(a.bias_offsets, a.bias_offset_bytes, row + 1);
     }
     const float repetition = a.repetition ? a.repetition[row] : a.repetition_value;
     const float presence = a.presence ? a.presence[row] : a.presence_value;
     const float frequency = a.frequency ? a.frequency[row] : a.frequency_value;
-    if (history || biases) {
+    auto clear = [&]() {
         for (int i = threadIdx.x * 4; i < TILE; i += T * 4)
             *reinterpret_cast<uint4 *>(words + i) = uint4{0, 0, 0, 0};
-        if (threadIdx.x == 0)
-            pair_count = 0;
         __syncthreads();
-    }
+    };
+    float f[kVecs][kItems];
     if (history) {
+        clear();
         begin = nbh_row_clamp(begin, 0, a.n_tokens);
         end = nbh_row_clamp(end, begin, a.n_tokens);
         const int prompt = (int)nbh_row_clamp(prompt_length, 0, end - begin);
@@ -152,68 +149,67 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
             else
                 atomicAdd(&words[t], 1u);
         });
+        __syncthreads();
     }
-    if (biases) {
+#pragma unroll
+    for (int j = 0; j < kVecs; ++j) {
+        const int at = (j * T + threadIdx.x) * kItems;
+        In::unpack(raw[j], f[j]);
+        if (!history || at >= n)
+            continue;
+        uint32_t word[kItems], any = 0;
+        for (int i = 0; i < kItems; ++i) {
+            word[i] = words[at + i];
+            any |= word[i];
+        }
+        if (any)
+            for (int i = 0; i < kItems; ++i) {
+                if (!word[i])
+                    continue;
+                const uint32_t count = word[i] & kCount;
+                float x = f[j][i];
+                x = x > 0.0f ? x / repetition : x * repetition;
+                if (count) {
+                    x = x - frequency * (float)count;
+                    x = x - presence;
+                }
+                f[j][i] = x;
+            }
+    }
+    if (BIASES) {
+        if (history)
+            __syncthreads();             // the words have been read
+        clear();
         pair0 = nbh_row_clamp(pair0, 0, a.n_bias);
         pair1 = nbh_row_clamp(pair1, pair0, a.n_bias);
-        visit_tokens<T>(a.bias_tokens, a.bias_token_bytes, pair0, pair1, first, n, [&](uint32_t t, int i) {
-            atomicOr(&words[t], kBiased);
-            const uint32_t place = atomicAdd(&pair_count, 1u);
-            if (place < kPairs) {
-                pair_at[place] = t;
-                pair_number[place] = (uint32_t)i;
-            }
-        });
-    }
-    if (history || biases)
+        visit_tokens<T>(a.bias_tokens, a.bias_token_bytes, pair0, pair1, first, n,
+                        [&](uint32_t t, int i) { atomicMax(&words[t], (uint32_t)i + 1); });
         __syncthreads();
+    }
 
     typename Out::item *out = reinterpret_cast<typename Out::item *>(a.out + row * a.out_stride) + first;
-
 #pragma unroll
     for (int j = 0; j < kVecs; ++j) {
         const int at = (j * T + threadIdx.x) * kItems;
         if (at >= n)
             break;
-        float f[kItems];
-        In::unpack(raw[j], f);
-        if (history || biases) {
-            uint32_t word[kItems], any = 0;
+        if (BIASES) {
+            uint32_t pair[kItems], any = 0;
             for (int i = 0; i < kItems; ++i) {
-                word[i] = words[at + i];
-                any |= word[i];
+                pair[i] = words[at + i];
+                any |= pair[i];
             }
-            if (any)
-                for (int i = 0; i < kItems; ++i) {
-                    if (!word[i])
-                        continue;
-                    const uint32_t count = word[i] & kCount;
-                    float x = f[i];
-                    if (word[i] & kSeen || count)
-                        x = x > 0.0f ? x / repetition : x * repetition;
-                    if (count) {
-                        x = x - frequency * (float)count;
-                        x = x - presence;
-                    }
-                    if (word[i] & kBiased) {
-                        int64_t last = -1;
-                        if (pair_count <= kPairs) {
-                            for (uint32_t k = 0; k < pair_count; ++k)
-                                if (pair_at[k] == (uint32_t)(at + i) && (int64_t)pair_number[k] > last)
-                                    last = pair_number[k];
-                        } else {
-                            for (int64_t k = pair1 - pair0; last < 0 && k-- > 0;)
-                                if (nbh_row_int(a.bias_tokens, a.bias_token_bytes, pair0 + k) == first + at + i)
-                                    last = k;
-                        }
-                        x = x + a.bias_values[pair0 + last];
-                    }
-                    f[i] = x;
-                }
+            if (any) {
+                float bias[kItems];      // all on their way at once; there is at least one pair
+                for (int i = 0; i < kItems; ++i)
+                    bias[i] = a.bias_values[pair[i] ? pair0 + pair[i] - 1 : 0];
+                for (int i = 0; i < kItems; ++i)
+                    f[j][i] = pair[i] ? f[j][i] + bias[i] : f[j][i];
+            }
         }
         for (int i = 0; i < kItems; ++i)
-            f[i] = bits[j] >> i & 1u ? f[i] : -INFINITY;
-        nbh_row_store<Out, true>(out, at, n, f);
+            f[j][i] = bits[j] >> i & 1u ? f[j][i] : -INFINITY;
+        nbh_row_store<Out, true>(out, at, n, f[j]);
     }
 }
 
@@ -225,7 +221,10 @@ int launch_adjust(Adjust a, int64_t rows, hipStream_t stream)
     const int64_t most = NBH_ROW_MOST_GROUPS / a.tiles;
     for (a.row0 = 0; a.row0 < rows; a.row0 += most) {
         const int64_t groups = (rows - a.row0 < most ? rows - a.row0 : most) * a.tiles;
-        adjust_rows<In, Out, T, TILE><<<dim3((unsigned)groups), dim3(T), 0, stream>>>(a);
+        if (a.bias_tokens)
+            adjust_rows<In, Out, T, TILE, true><<<dim3((unsigned)groups), dim3(T), 0, stream>>>(a);
+        else
+            adjust_rows<In, Out, T, TILE, false><<<dim3((unsigned)groups), dim3(T), 0, stream>>>(a);
         if (const int status = nbh_launch_status())
             return status;
     }

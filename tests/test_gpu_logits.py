@@ -461,3 +461,9 @@ def test_top_of_many_masked_rows(k):
     order = np.argsort(-a, axis=1, kind="stable")[:, :k]
     assert np.array_equal(indices, order)
     assert np.array_equal(values, np.take_along_axis(a, order, 1))
+
+
+@pytest.mark.parametrize("name", cases.DTYPES)
+@pytest.mark.parametrize("rows, vocab, longest, pairs", [(4, 900, 50, 5000), (3, 9000, 0, 9000), (2, 5000, 40000, 3000)])
+def test_adjust_with_biases_for_all(name, rows, vocab, longest, pairs):
+    cases.check_adjust(cuda, rows, vocab, name, name, longest, pairs, "rows")
