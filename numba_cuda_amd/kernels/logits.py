@@ -59,7 +59,8 @@ _INTEGERS = {devicearray.DeviceNDArray: False, _int32: (4, 4), _int64: (8, 8)}
 _FLOATS = {devicearray.DeviceNDArray: False, _float32: (4, 0)}
 _TABLES = (_ROWS, _INTEGER_ROWS, _INT32_ROWS, _WORDS, _INTEGERS, _FLOATS)
 
-_row_view, _vector_view = _driver._hostbuf.row_view, _driver._hostbuf.vector_view
+_row_view = getattr(_driver._hostbuf, "row_view", lambda *_: None)         # None from an older build: slower
+_vector_view = getattr(_driver._hostbuf, "vector_view", lambda *_: None)
 
 _foreign_dtypes = {}                         # dtype objects of other libraries -> np.dtype
 
