@@ -661,12 +661,15 @@ Spread spread_of(int64_t rows, int64_t vocab, int dtype, int spare)
 //   44 and 50, 4096 x 32768 118 and 180, 1024 x 50021 57 and 66, 512 x 131072 66 and 51 (k = 300: 2048 x 131072
 //   159 and 143).
 //   k = 1000: 4096 x 1024 117 and 214, 4096 x 8192 222 and 391, 4096 x 32768 799 and 265 (k = 700: 395 and 214).
+//   k > 512, few short rows: 45 x 1822, k = 981, 40 and 19, 512 x 8192, k = 700, 38 and 29, 900 x 8192, k = 600,
+//   41 and 48, 900 x 4096, k = 1000, 60 and 64.
 int lanes_of(int64_t rows, int64_t vocab, int64_t bytes, int k)
 {
     const bool brief = vocab * bytes <= (16 << 10);
     if (brief && k <= 64 && rows >= 2048)
         return 64;
-    if (brief || k <= 256 || (k <= 512 && rows >= 1024 && vocab * bytes <= (128 << 10)))
+    if (k <= 256 || (brief && (k <= 512 || rows > 512)) ||
+        (k <= 512 && rows >= 1024 && vocab * bytes <= (128 << 10)))
         return 256;
     return 512;
 }
