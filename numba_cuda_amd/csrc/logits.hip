@@ -15,7 +15,7 @@
 // Bound by memory where rows are many, by the start of a launch and the walk through the history where they are
 // few.  256 x 131072 bfloat16 to float32 with masks, 64 biases and histories of 4096 a row: 42 us, its 208 MB at
 // 4.9 TB/s (72 us while results of four bytes left a lane in two stores 16 bytes apart, hence the half vectors; 98
-// us with inputs read past the caches).
+// us with inputs read past the caches).  8 x 131072 float32 with histories of 131071: 15.5 us, each tile's walk.
 #include "rows.h"
 
 namespace {
@@ -100,8 +100,8 @@ __global__ __launch_bounds__(T) void adjust_rows(Adjust a)
     constexpr int kItems = In::items, kVecs = TILE / (T * kItems);
     static_assert(Out::items == kItems, "as many entries per vector on both sides");
     __shared__ uint32_t words[TILE];
-    // Rows first, so that where there are eight rows or a multiple all tiles of one run on one XCD, whose L2 then holds
-    // its history alone (8 x 131072 float32, histories of 131071: 15.5 us, tiles first 16.8; 64 x 50021 7.9 and 8.7).
+    // Rows first (8 x 131072 float32, histories of 131071: 15.5 us, tiles first 16.8; 64 x 50021 float16 7.9 and
+    // 8.7; 256 x 131072 42 either way).
     const uint32_t now = gridDim.x / a.tiles;
     const int64_t row = a.row0 + blockIdx.x % now;
     const int tile = blockIdx.x / now;

@@ -15,8 +15,9 @@
 // Short rows: one workgroup does all of that for a row.  Long ones: a first launch of small workgroups in the
 // order of memory finds the groups' maxima and the statistics of the log-sum-exp, a second one does the rest.
 // For many rows one launch is faster, as one row's bisection hides behind another's reading: 4096 x 65536
-// bfloat16, k = 64, 110 us (537 MB at 4.9 TB/s), in two launches 103 + 53.  Few long rows end with the second
-// launch's latency: 16 x 131072 float16, k = 512, 5 + 15 us; 64 x 100003 bfloat16, k = 50, 8 + 10 us.
+// bfloat16, k = 64, 116 us (537 MB at 4.6 TB/s; 676 MB leave the L2 caches, with the lines read again), in two
+// launches 103 + 53.  Few long rows end with the second launch's latency: 16 x 131072 float16, k = 512, 5 + 19 us;
+// 64 x 100003 bfloat16, k = 50, 9 + 11 us.
 #include "rows.h"
 
 namespace {
