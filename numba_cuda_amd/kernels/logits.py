@@ -253,7 +253,7 @@ def _result_numbers(obj, name, rows, stream, handle):
     return obj, _vector_of(obj, name, rows, stream, _FLOATS, output=True)[0]
 
 
-def _workspace(given, nbytes, handle):
+def _workspace(given, nbytes, handle, others):
     """(address, bytes, what keeps it alive)."""
     if given is not None:
         address, shape, strides, dtype, owner = _checked_view(given, "workspace", 0, output=True)
@@ -264,6 +264,8 @@ def _workspace(given, nbytes, handle):
             expect *= n
         if expect < nbytes or address % 16:
             raise ValueError("workspace must hold %d bytes, aligned to 16" % nbytes)
+        if nbytes:
+            _refuse_overlaps([(address, 1, nbytes, 0, "workspace")], others)
         return address, expect, owner
     if not nbytes:
         return _NO_WORKSPACE
@@ -333,6 +335,9 @@ def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, 
     x = (address, rows, vocab * _SIZE[code], in_stride, "logits")
     _refuse_overlaps([(y[0], rows, vocab * _SIZE[y[4]], y[3], "out")], [x], same=x)
 
+    low = high = 0                           # the bytes `out` lies in: no other array may touch them
+    if rows and vocab:
+        low, high = y[0] + min(0, (rows - 1) * y[3]), y[0] + max(0, (rows - 1) * y[3]) + vocab * _SIZE[y[4]]
     history, bias = _NO_HISTORY, _NO_BIAS
     if tokens is not None:
         t = _vector_of(tokens, "tokens", None, stream, _INTEGERS, keep=keep)
@@ -344,14 +349,26 @@ def adjust(logits, out=None, *, tokens=None, offsets=None, prompt_lengths=None, 
         pre = _per_row(presence, "presence", rows, stream, 0.0, keep)
         fre = _per_row(frequency, "frequency", rows, stream, 0.0, keep)
         history = (t[0], o[0], p[0], t[1], t[2], o[2], p[2], rep[0], pre[0], fre[0], rep[1], pre[1], fre[1])
+        if (t[0] < high and low < t[0] + t[1] * t[2]) or (o[0] < high and low < o[0] + (rows + 1) * o[2]) or (
+                p[0] < high and low < p[0] + rows * p[2]) or (rep[0] < high and low < rep[0] + rows * 4) or (
+                pre[0] < high and low < pre[0] + rows * 4) or (fre[0] < high and low < fre[0] + rows * 4):
+            raise ValueError("out overlaps the history or the penalties")
     if bias_tokens is not None:
         t = _vector_of(bias_tokens, "bias_tokens", None, stream, _INTEGERS, keep=keep)
         v = _vector_of(bias_values, "bias_values", t[1], stream, _FLOATS, np.float32, keep=keep)
         o = _vector_of(bias_offsets, "bias_offsets", rows + 1, stream, _INTEGERS, keep=keep)
         bias = (t[0], o[0], v[0], t[1], t[2], o[2])
+        if (t[0] < high and low < t[0] + t[1] * t[2]) or (v[0] < high and low < v[0] + t[1] * 4) or (
+                o[0] < high and low < o[0] + (rows + 1) * o[2]):
+            raise ValueError("out overlaps the biases")
     mask_address = mask_stride = 0
     if mask is not None:
         mask_address, mask_stride = _mask_of(mask, rows, vocab, stream, keep)
+        words = (vocab + 31) // 32 * 4
+        if rows and vocab and mask_address + min(0, mask_stride * (rows - 1)) < high and (
+                low < mask_address + max(0, mask_stride * (rows - 1)) + words) and not _beside(
+                (y[0], rows, vocab * _SIZE[y[4]], y[3]), (mask_address, rows, words, mask_stride)):
+            raise ValueError("out overlaps mask")
 
     if rows and vocab:
         _driver.driver.nbh_logits_adjust(
@@ -440,9 +457,11 @@ def top(logits, k, *, values=None, indices=None, lse=None, temperature=1.0, work
     if wanted:
         lse, lse_address = _result_numbers(lse, "lse", rows, stream, handle)
         results.append((lse_address, 1, rows * 4, 0, "lse"))
-    _refuse_overlaps(results, [(address, rows, vocab * _SIZE[code], stride, "logits")])
+    inputs = [(address, rows, vocab * _SIZE[code], stride, "logits")]
+    _refuse_overlaps(results, inputs)
     if rows:
-        space = _workspace(workspace, _driver.driver.lib.nbh_rows_top_workspace(rows, vocab, k, code), handle)
+        space = _workspace(workspace, _driver.driver.lib.nbh_rows_top_workspace(rows, vocab, k, code), handle,
+                           results + inputs)
         _launch(space, _driver.driver.nbh_rows_top, address, rows, vocab, stride, code, k, v[0], v[3], i[0], i[3],
                 lse_address, temperature, space[0] or None, space[1], handle or None)
     return (values, indices, lse) if wanted else (values, indices)
@@ -502,7 +521,8 @@ def _distill(what, grad_loss, student, values, indices, temperature, teacher_lse
     _refuse_overlaps(results, inputs, same=x)
 
     if rows:
-        space = _workspace(workspace, _driver.driver.lib.nbh_rows_distill_workspace(rows, vocab, k, code, what), handle)
+        space = _workspace(workspace, _driver.driver.lib.nbh_rows_distill_workspace(rows, vocab, k, code, what), handle,
+                           results + inputs)
         arguments = _DISTILL.pack(_DISTILL_SIZE, what, address, rows, vocab, stride, code, v[0], i[0], k, v[3], v[4], i[3],
                                   i[4], teacher_address, grad_address, grad_stride, grad_value, temperature,
                                   loss_address, lse_address, out_address, out_stride, space[0], space[1])

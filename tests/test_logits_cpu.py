@@ -252,3 +252,45 @@ def test_the_entry_points_check_their_arguments():
     # long rows are spread over workgroups, short ones are not
     assert lib.nbh_rows_top_workspace(1, 131072, 50, 0) > 0 == lib.nbh_rows_top_workspace(4096, 1000, 50, 0)
     assert lib.nbh_rows_distill_workspace(1, 1310720, 8, 2, 1) > 0 == lib.nbh_rows_distill_workspace(1, 131072, 8, 2, 2)
+
+
+def test_results_may_not_touch_any_other_argument(fake_gpu, monkeypatch):
+    launched = []
+    monkeypatch.setattr(fake_gpu, "nbh_logits_adjust", lambda *a: launched.append(a) or 0, raising=False)
+    block = cuda.to_device(np.zeros(4096, np.float32))
+
+    def part(first, shape, dtype):
+        strides = tuple(np.zeros(shape, dtype).strides)
+        return devicearray.DeviceNDArray(shape, strides, np.dtype(dtype), gpu_data=block[first:].gpu_data)
+
+    x, out = _f32(2, 40), part(100, (2, 40), np.float32)                 # floats 100 .. 179 of the block
+    tokens, offsets, values = _i32(10), _i32(3), _f32(10)
+    for kw in (dict(tokens=part(95, (10,), np.int32), offsets=offsets), dict(tokens=tokens, offsets=part(179, (3,), np.int32)),
+               dict(tokens=tokens, offsets=offsets, prompt_lengths=part(120, (2,), np.int32)),
+               dict(tokens=tokens, offsets=offsets, repetition=part(99, (2,), np.float32)),
+               dict(tokens=tokens, offsets=offsets, presence=part(140, (2,), np.float32)),
+               dict(tokens=tokens, offsets=offsets, frequency=part(178, (2,), np.float32))):
+        with pytest.raises(ValueError, match="out overlaps the history or the penalties"):
+            logits.adjust(x, out, **kw)
+    for kw in (dict(bias_tokens=part(91, (10,), np.int32), bias_values=values, bias_offsets=offsets),
+               dict(bias_tokens=tokens, bias_values=part(170, (10,), np.float32), bias_offsets=offsets),
+               dict(bias_tokens=tokens, bias_values=values, bias_offsets=part(98, (3,), np.int32))):
+        with pytest.raises(ValueError, match="out overlaps the biases"):
+            logits.adjust(x, out, **kw)
+    for mask in (part(97, (2, 2), np.int32), part(99, (2,), np.int32), part(179, (2, 2), np.int32)):
+        with pytest.raises(ValueError, match="out overlaps mask"):
+            logits.adjust(x, out, mask=mask)
+    assert not launched
+    # on either side of it
+    logits.adjust(x, out, tokens=part(90, (10,), np.int32), offsets=part(180, (3,), np.int32), mask=part(96, (2, 2), np.int32))
+    assert len(launched) == 1
+
+
+def test_a_workspace_may_not_touch_the_other_arguments(fake_gpu, monkeypatch):
+    monkeypatch.setattr(fake_gpu, "nbh_rows_top_workspace", lambda *a: 64, raising=False)
+    monkeypatch.setattr(fake_gpu, "nbh_rows_distill_workspace", lambda *a: 64, raising=False)
+    x, v, i = _f32(2, 40), _f32(2, 3), _i32(2, 3)
+    with pytest.raises(ValueError, match="workspace overlaps logits"):
+        logits.top(x, 3, workspace=x)
+    with pytest.raises(ValueError, match="workspace overlaps student"):
+        logits.distill_loss(x, v, i, workspace=x)
