@@ -529,7 +529,10 @@ template <typename E> __global__ __launch_bounds__(256) void distill_named(Disti
 // 8192 40, 40 and 74.  In several launches: loss 131072 x 1024 280 instead of 171, 16384 x 8192 70 instead of 59,
 // gradient 288 instead of 234 and 153 instead of 137.
 // Both at once, 256 and 512 lanes: 4096 x 16384 67 and 97, 4096 x 32768 125 and 130, 512 x 16384 17 and 17, 256 x
-// 32768 18 and 17, 4096 x 50021 242 and 224, 4096 x 65536 244 and 209.
+// 32768 18 and 17, 4096 x 50021 242 and 224, 4096 x 65536 244 and 209.  With many entries of the teacher, whose LDS
+// leaves room for one workgroup of 512 only and which take a wavefront long: 4096 x 65536, k = 150 267 and 256, 300
+// 299 and 317, 500 347 and 415, 600 371 and 627, 1000 457 and 906; 1024 x 131072, k = 300 149 and 137, 500 166 and
+// 174, 1000 205 and 287; 256 x 131072, k = 1000 77 and 71.
 enum Way { kRows, kInParts, kFlat };
 struct Spread {
     Way way;
@@ -537,7 +540,7 @@ struct Spread {
     int64_t slice;
 };
 // `spare`: entries before a row's beginning that its first vector may hold
-Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what, int spare)
+Spread spread_of(int64_t rows, int64_t vocab, int64_t k, int dtype, int what, int spare)
 {
     const int64_t items = dtype == NBH_ROW_F32 ? 4 : 8;
     const int64_t chunk = 256 * kNbhAhead * items;           // 16 KiB, a step of the row kernel
@@ -550,8 +553,10 @@ Spread spread_of(int64_t rows, int64_t vocab, int dtype, int what, int spare)
         return {kFlat, (int)((vocab + spare + flat - 1) / flat), 0, 1, vocab};
     if (what == kLoss)
         return {large || (rows < 256 && chunks > 24) ? kInParts : kRows, tiles, small ? 64 : 256, 1, vocab};
-    if (what == (kLoss | kGrad) && (rows >= 128 || chunks <= 12))
-        return {kRows, tiles, small ? 64 : chunks <= 4 && rows > 512 ? 256 : 512, 1, vocab};
+    if (what == (kLoss | kGrad) && (rows >= 128 || chunks <= 12)) {
+        const bool more = (chunks <= 4 && rows > 512) || (k > 512 && rows > 256);
+        return {kRows, tiles, small ? 64 : more ? 256 : 512, 1, vocab};
+    }
     int64_t splits = (1024 + rows - 1) / rows;
     if (splits > chunks)
         splits = chunks;
@@ -610,7 +615,7 @@ extern "C" size_t nbh_rows_distill_workspace(int64_t rows, int64_t vocab, int64_
     if (rows <= 0 || vocab < 0 || vocab > INT32_MAX || k < 0 || k > NBH_ROW_TOP_MOST || dtype < 0 ||
         dtype > NBH_ROW_BF16 || what < kLoss || what > (kLoss | kGrad))
         return 0;
-    const Spread s = spread_of(rows, vocab, dtype, what, 7);
+    const Spread s = spread_of(rows, vocab, k, dtype, what, 7);
     if (s.way == kFlat)
         return (size_t)rows * (sizeof(Plan) + (size_t)k * sizeof(Named));
     if (s.way == kInParts)
@@ -635,7 +640,7 @@ extern "C" int nbh_rows_distill(const struct nbh_rows_distill_args *p, nbh_strea
     const size_t need = nbh_rows_distill_workspace(p->rows, p->vocab, p->k, (int)p->dtype, (int)p->what);
     if (need && (!p->workspace || p->workspace_bytes < (int64_t)need || ((uintptr_t)p->workspace & 15)))
         return (int)hipErrorInvalidValue;
-    const Spread spread = spread_of(p->rows, p->vocab, (int)p->dtype, (int)p->what,
+    const Spread spread = spread_of(p->rows, p->vocab, p->k, (int)p->dtype, (int)p->what,
                                     nbh_row_spare(p->student, p->stride, (int)p->dtype));
     Distill a = {};
     a.student = (const char *)p->student;

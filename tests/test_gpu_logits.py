@@ -467,3 +467,8 @@ def test_top_of_many_masked_rows(k):
 @pytest.mark.parametrize("rows, vocab, longest, pairs", [(4, 900, 50, 5000), (3, 9000, 0, 9000), (2, 5000, 40000, 3000)])
 def test_adjust_with_biases_for_all(name, rows, vocab, longest, pairs):
     cases.check_adjust(cuda, rows, vocab, name, name, longest, pairs, "rows")
+
+
+@pytest.mark.parametrize("name", ["float32", "bfloat16"])
+def test_distill_of_many_rows_and_entries(name):
+    cases.check_distill(cuda, 300, 33000, name, 600, what="both", pad=3)
