@@ -25,10 +25,10 @@ constexpr int kStatsThreads = 64, kStatsVecs = 8;      // 8 KiB per workgroup
 constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596299e-8f;       // log2(e) and its rounding
 constexpr float kLn2 = 0.693147180559945309f;
 
-// exp(s / T - lse) P grad_loss / T = whole * 2^(s * scale - peak * scale) for a row; 0 where `zero`.
+// exp(s / T - lse) P grad_loss / T = whole * nbh_softmax_term(s, peak, scale, shift) for a row; 0 where `zero`.
 struct Plan {
-    float peak, whole;
-    int zero, unused;
+    float peak, whole, shift;
+    int zero;
 };
 // An entry of the gradient that the teacher names: its index (-1: none) and value.
 struct Named {
@@ -157,7 +157,7 @@ struct Teacher {
 // One wavefront's work: no barriers, its LDS accesses are in order.  `begin` .. `end`: the part of the row
 // whose values are wanted (elsewhere another workgroup may be writing the gradient over them already).
 template <typename E, int WHAT>
-__device__ void load_teacher(const Distill &a, int64_t row, int64_t begin, int64_t end, Teacher &t)
+__device__ __forceinline__ void load_teacher(const Distill &a, int64_t row, int64_t begin, int64_t end, Teacher &t)
 {
     const typename E::item *in = reinterpret_cast<const typename E::item *>(a.student + row * a.stride);
     const int lane = threadIdx.x & 63;
@@ -220,31 +220,36 @@ __device__ void load_teacher(const Distill &a, int64_t row, int64_t begin, int64
     t.repeated = __any(repeated);
 }
 
-// The student's side of a row: q(v) = base * 2^(s scale - peak scale).
+// The student's side of a row: q(v) = base * nbh_softmax_term(s, peak, scale, shift).
 struct Student {
     float peak, base, log_sum;           // log_sum: log2 of the sum relative to the peak
+    float shift;
 };
 __device__ __forceinline__ Student student_of(nbh_softmax stats)
 {
-    return {stats.peak == -INFINITY ? 0.0f : stats.peak, stats.sum == 0.0f ? 0.0f : 1.0f / stats.sum, log2f(stats.sum)};
+    return {stats.peak == -INFINITY ? 0.0f : stats.peak, stats.sum == 0.0f ? 0.0f : 1.0f / stats.sum, log2f(stats.sum),
+            0.0f};
 }
 __device__ __forceinline__ Student student_of_lse(const Distill &a, float lse)
 {
     // T * lse rounded to float32 takes the place of the peak; what the roundings of it, of its product
-    // with the scale, and of the scale itself take off goes into the factor.
+    // with the scale, and of the scale itself take off goes into the factor.  Where the product is not near, the
+    // first of them may be hundreds of powers of two, which only together with the difference s - peak make an
+    // ordinary exponent.
     const float peak = lse * a.temperature, product = peak * a.scale;
     if (lse == -INFINITY)
-        return {0.0f, 0.0f, 0.0f};
+        return {0.0f, 0.0f, 0.0f, 0.0f};
     if (nbh_softmax_near(product)) {
         const float high = lse * kLog2e, low = fmaf(lse, kLog2e, -high) + lse * kLog2eRest;
-        return {peak, exp2f((product - high) - low + peak * a.scale_rest), 0.0f};
+        return {peak, exp2f((product - high) - low + peak * a.scale_rest), 0.0f, 0.0f};
     }
     const float rest = __builtin_isfinite(peak) ? fmaf(lse, a.temperature, -peak) : 0.0f;
-    return {peak, expf(-rest / a.temperature), 0.0f};
+    // the same for the whole row: in a scalar register
+    return {peak, 1.0f, 0.0f, __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(rest * a.scale)))};
 }
 
-// One wavefront's work.
-__device__ float loss_of(const Distill &a, const Teacher &t, Student s)
+// One wavefront's work.  (Called, not inlined, it would leave the arguments in scratch memory.)
+__device__ __forceinline__ float loss_of(const Distill &a, const Teacher &t, Student s)
 {
     const float product = s.peak * a.scale;
     float loss = 0.0f;
@@ -287,7 +292,7 @@ __device__ __forceinline__ Named named_of(const Distill &a, const Teacher &t, in
             if (t.index[i] == index)
                 own += t.p[i];
     }
-    return {index, whole * nbh_softmax_term(t.student[j], s.peak, a.scale) - factor * own};
+    return {index, whole * nbh_softmax_term(t.student[j], s.peak, a.scale, s.shift) - factor * own};
 }
 
 // With 512 lanes the loss and the gradient together keep the beginning of the row, 96 KiB of it in registers and
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(T, (Kept<T, WHAT>::waves)) void distill_rows(Distil
                     f[i] = whole * nbh_exp2(fmaf(f[i], a.scale, -product));
             } else {
                 for (int i = 0; i < kItems; ++i)
-                    f[i] = whole * nbh_exp2((f[i] - student.peak) * a.scale);
+                    f[i] = whole * nbh_exp2((f[i] - student.peak) * a.scale - student.shift);
             }
             nbh_row_store<E, true>(out, at + (j * T + threadIdx.x) * kItems, end, f);
         }
@@ -450,7 +455,7 @@ template <typename E> __global__ __launch_bounds__(64) void distill_plan(Distill
     const bool zero = !teacher.some || factor == 0.0f;
     const float whole = factor * teacher.mass * student.base;
     if (threadIdx.x == 0)
-        a.plans[row - a.row0] = {student.peak, whole, zero, 0};
+        a.plans[row - a.row0] = {student.peak, whole, student.shift, zero};
     for (int j = threadIdx.x; j < a.k; j += 64)
         a.named[(row - a.row0) * a.k + j] = zero ? Named{-1, 0.0f} : named_of(a, teacher, j, student, whole, factor);
 }
@@ -490,7 +495,7 @@ template <typename E> __global__ __launch_bounds__(kFlatThreads) void distill_fl
                 f[i] = plan.whole * nbh_exp2(fmaf(f[i], a.scale, -product));
         } else {
             for (int i = 0; i < kItems; ++i)
-                f[i] = plan.whole * nbh_exp2((f[i] - plan.peak) * a.scale);
+                f[i] = plan.whole * nbh_exp2((f[i] - plan.peak) * a.scale - plan.shift);
         }
         const int64_t at = first + (j * T + (int)threadIdx.x) * kItems;
         if (full)

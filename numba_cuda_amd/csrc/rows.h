@@ -169,46 +169,60 @@ __device__ __forceinline__ void nbh_row_store(typename E::item *row, int64_t at,
 }
 
 // Running softmax statistics of values x, with scale = log2(e) / temperature: `sum` is the sum of
-// 2^(x scale - peak scale) for a reference `peak` (-inf before the first value above -inf), which is at
-// most 64 powers of two below the largest value: it is raised only when a value would exceed that, so that
-// nearly all values cost one fused multiply-add, one exponential and one addition.  The product peak scale
-// is rounded once and used so everywhere, which makes the rounding harmless.  Where it would overflow
-// (rows filled with the type's lowest value) differences x - peak are formed first instead.
+// 2^(x scale - origin) for a reference `peak` (-inf before the first value above -inf), which is at
+// most 32 powers of two below the largest value: it is raised only when a value would exceed that, so that
+// nearly all values cost one fused multiply-add, one exponential and one addition.
+// The origin is peak scale.  Below 2^22 it is that product rounded once, which the rounding moves by at most a
+// quarter: used so everywhere, that is harmless.  Beyond, the rounding would take whole powers of two off
+// (masked rows, tiny temperatures), so the origin is the exact product there and the terms are
+// 2^((x - peak) scale).  Where a step of float32 at the peak is as large as the 32 powers of two, rounding may let
+// a value of up to 64 pass: 2^31 of them still add up to a finite sum.
 // A NaN stays in `sum`; a row of -inf has peak -inf and sum 0; +inf makes `sum` inf.
 struct nbh_softmax {
     float peak, sum;
 };
 __device__ __forceinline__ nbh_softmax nbh_softmax_empty() { return {-INFINITY, 0.0f}; }
 __device__ __forceinline__ float nbh_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ __forceinline__ bool nbh_softmax_near(float product) { return fabsf(product) < 1e30f; }
-// 2^(x scale - peak scale)
-__device__ __forceinline__ float nbh_softmax_term(float x, float peak, float scale)
+__device__ __forceinline__ bool nbh_softmax_near(float product) { return fabsf(product) < 0x1p22f; }
+// 2^(x scale - origin of peak - shift); `shift` counts only where that product is not near.
+__device__ __forceinline__ float nbh_softmax_term(float x, float peak, float scale, float shift = 0.0f)
 {
     const float product = peak * scale;
-    return nbh_exp2(nbh_softmax_near(product) ? fmaf(x, scale, -product) : (x - peak) * scale);
+    return nbh_exp2(nbh_softmax_near(product) ? fmaf(x, scale, -product) : (x - peak) * scale - shift);
 }
+// What rounding took off the product that is the origin.
+__device__ __forceinline__ float nbh_softmax_rest(float peak, float scale)
+{
+    const float product = peak * scale;
+    return nbh_softmax_near(product) ? fmaf(peak, scale, -product) : 0.0f;
+}
+// 2^(origin of one peak - origin of another)
 __device__ __forceinline__ float nbh_softmax_factor(float from, float to, float scale)
 {
     const float a = from * scale, b = to * scale;
-    return nbh_exp2(nbh_softmax_near(a) && nbh_softmax_near(b) ? a - b : (from - to) * scale);
+    return nbh_exp2(nbh_softmax_near(a) && nbh_softmax_near(b)
+                        ? a - b
+                        : (from - to) * scale - nbh_softmax_rest(from, scale) + nbh_softmax_rest(to, scale));
 }
 // Values f, the largest of which is `most` (or NaN).
 template <int N>
 __device__ __forceinline__ void nbh_softmax_add(nbh_softmax &s, const float (&f)[N], float most, float scale)
 {
-    // 64 powers of two above the reference
-    if (__any(!(most <= fmaf(64.0f, __builtin_amdgcn_rcpf(scale), s.peak)))) {
+    // 32 powers of two above the reference
+    if (__any(!(most <= fmaf(32.0f, __builtin_amdgcn_rcpf(scale), s.peak)))) {
         const float peak = fmaxf(s.peak, fminf(most, FLT_MAX));
         if (peak != s.peak) {
-            s.sum *= nbh_softmax_factor(s.peak, peak, scale);
+            s.sum *= nbh_exp2((s.peak - peak) * scale - nbh_softmax_rest(s.peak, scale) + nbh_softmax_rest(peak, scale));
             s.peak = peak;
         }
     }
     const float product = s.peak == -INFINITY ? 0.0f : s.peak * scale;
     float sum[2] = {0.0f, 0.0f};
     if (__any(!nbh_softmax_near(product))) {
+        // for all lanes of the wavefront, those of which the product is near too
+        const float peak = s.peak == -INFINITY ? 0.0f : s.peak, rest = nbh_softmax_rest(peak, scale);
         for (int i = 0; i < N; ++i)
-            sum[i & 1] += s.peak == -INFINITY ? nbh_exp2(f[i]) : nbh_softmax_term(f[i], s.peak, scale);
+            sum[i & 1] += nbh_exp2((f[i] - peak) * scale + rest);
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -238,14 +252,21 @@ __device__ __forceinline__ float nbh_softmax_lse(nbh_softmax s, float temperatur
     return nbh_softmax_near(product) ? (product + log2f(s.sum)) * 0.693147180559945309f
                                      : s.peak / temperature + logf(s.sum);
 }
-// Over a wavefront; every lane gets the result.
+// The sum for the reference `peak`, which is not below its own.
+__device__ __forceinline__ float nbh_softmax_raised(nbh_softmax s, float peak, float scale)
+{
+    return peak == -INFINITY ? s.sum : s.sum * nbh_softmax_factor(s.peak, peak, scale);
+}
+// Over a wavefront, whose lanes' sums are brought to one reference first; every lane gets the result.
 __device__ __forceinline__ nbh_softmax nbh_softmax_wave(nbh_softmax s, float scale)
 {
-    for (int step = 32; step; step >>= 1) {
-        const nbh_softmax other = {__shfl_xor(s.peak, step), __shfl_xor(s.sum, step)};
-        s = nbh_softmax_join(s, other, scale);
-    }
-    return s;
+    float peak = s.peak;
+    for (int step = 32; step; step >>= 1)
+        peak = fmaxf(peak, __shfl_xor(peak, step));
+    float sum = nbh_softmax_raised(s, peak, scale);
+    for (int step = 32; step; step >>= 1)
+        sum += __shfl_xor(sum, step);
+    return {peak, sum};
 }
 // Over a workgroup of `T` lanes; `room` holds T / 64 entries.  Every lane gets the result.
 template <int T>
@@ -255,10 +276,14 @@ __device__ __forceinline__ nbh_softmax nbh_softmax_group(nbh_softmax s, float sc
     if ((threadIdx.x & 63) == 0)
         room[threadIdx.x >> 6] = s;
     __syncthreads();
-    s = room[0];
+    if (T == 64)
+        return s;
+    float peak = room[0].peak, sum = 0.0f;
     for (int w = 1; w < T / 64; ++w)
-        s = nbh_softmax_join(s, room[w], scale);
-    return s;
+        peak = fmaxf(peak, room[w].peak);
+    for (int w = 0; w < T / 64; ++w)
+        sum += nbh_softmax_raised(room[w], peak, scale);
+    return {peak, sum};
 }
 
 // A workgroup of T lanes goes through elements begin .. end of a row in chunks of `kNbhAhead` 16-byte
