@@ -236,14 +236,19 @@ def _distill(with_loss, with_grad, grad_loss, student, values, indices, temperat
         if with_loss:
             peak, total = _softmax(line, temperature)
             norms[r] = peak / temperature + np.log(total)
+            q = np.exp((line - peak) / temperature) / (total if total else _f32(1))
             log_q = np.where(line[at] == -np.inf, line[at], (line[at] - peak) / temperature - np.log(total))
             losses[r] = np.where(p != 0, p * (log_p - log_q), _f32(0)).sum(dtype=_f32)
+        elif norms[r] == -np.inf:
+            q = np.zeros(vocab, _f32)
+        else:
+            # the difference in float64: in float32 the quotient alone is off by far more than one for large logits
+            q = np.exp(line / np.float64(temperature) - np.float64(norms[r])).astype(_f32)
         if with_grad:
             factor = grad_loss[r] / temperature
             if not len(at) or factor == 0:
                 grad = np.zeros(vocab, _f32)
             else:
-                q = np.zeros(vocab, _f32) if norms[r] == -np.inf else np.exp(line / temperature - norms[r])
                 grad = factor * p.sum(dtype=_f32) * q
                 np.add.at(grad, at, -factor * p)
             _store(y, r, grad)
