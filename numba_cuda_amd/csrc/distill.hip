@@ -554,7 +554,9 @@ Spread spread_of(int64_t rows, int64_t vocab, int64_t k, int dtype, int what, in
     const int64_t chunks = vocab ? (vocab + chunk - 1) / chunk : 1;
     const bool small = chunks == 1, large = !small && rows * vocab >= ((int64_t)128 << 20) / 16 * items;
     const int tiles = (int)((vocab + spare + tile - 1) / tile);
-    if (what == kGrad && large)
+    // kFlat needs a launch to hold a row (whatever `spare` is: the workspace goes by the largest); from 2^29
+    // entries of four bytes or 2^30 of two on, one does not.
+    if (what == kGrad && large && vocab + 7 <= (int64_t)NBH_ROW_MOST_GROUPS * flat)
         return {kFlat, (int)((vocab + spare + flat - 1) / flat), 0, 1, vocab};
     if (what == kLoss)
         return {large || (rows < 256 && chunks > 24) ? kInParts : kRows, tiles, small ? 64 : 256, 1, vocab};

@@ -12,8 +12,9 @@ typedef float nbh_f32x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 nbh_f16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 nbh_bf16x2 __attribute__((ext_vector_type(2)));
 
-// Workgroups of one launch: with up to 1024 lanes each they stay below 2^32 lanes.  2^31 entries of a row
-// make 2^19 tiles of 4096, so every row fits a launch.
+// Workgroups of one launch: with up to 1024 lanes each they stay below 2^32 lanes.  A row of 2^31 entries makes
+// 2^20 tiles of the statistics' 2048 float32 entries, fewer of every other kernel but the gradient's in the order of
+// memory, which takes 256 entries and is for rows that fit a launch.
 #define NBH_ROW_MOST_GROUPS (1 << 21)
 
 // Element types.  `items` elements make 16 bytes; arithmetic is float32 throughout, stores round once,
