@@ -19,7 +19,7 @@ of the item size apart.  Arithmetic is float32, results are rounded once.
 Everything is asynchronous on `stream`, and results do not depend on how the work was spread.  A call
 that needs a workspace keeps one per stream; a call recorded into a graph takes the caller's
 (`workspace=`, at least `top_workspace` / `distill_workspace` bytes) and the caller's result arrays,
-since a graph may run beside later calls on its stream.
+since a graph may run beside later calls on its stream, and inputs in device memory only.
 """
 
 import ctypes
@@ -118,6 +118,8 @@ def _checked_view(obj, name, stream, dtype=None, output=False):
     if view is None:
         if output:
             raise TypeError("%s must be a device array" % name)
+        if _capturing(_driver._stream_handle(stream)):       # each replay would copy from a host array that is gone
+            raise ValueError("a call that is captured into a graph needs %s in device memory" % name)
         host = np.ascontiguousarray(obj, dtype=dtype)
         view = _device_view(devicearray.auto_device(host, stream=stream)[0])
     if not _one_device() and view[0]:        # memory of another device than the calling thread's
