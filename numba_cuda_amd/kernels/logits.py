@@ -28,6 +28,7 @@ import struct
 
 import numpy as np
 
+from numba_cuda_amd._logits_host import beside as _beside, refuse_overlaps as _refuse_overlaps
 from numba_cuda_amd._logits_host import bfloat16, from_bfloat16, to_bfloat16  # noqa: F401
 from numba_cuda_amd.cudadrv import devicearray, devices
 from numba_cuda_amd.cudadrv import driver as _driver
@@ -177,33 +178,6 @@ def _vector_of(obj, name, length, stream, table, dtype=None, output=False, keep=
 
 
 _SIZE = (4, 2, 2)                            # item size by row code
-
-
-def _refuse_overlaps(results, inputs, same=None):
-    """ValueError when a result array touches an input or another result.  Both are lists of blocks
-    (address, rows, bytes of a row, bytes from row to row, name); `same`: the input that a result may
-    be, byte for byte."""
-    spans = []
-    for block in results + inputs:
-        address, rows, width, step, _ = block
-        reach = (rows - 1) * step
-        low, high = (address + reach, address + width) if reach < 0 else (address, address + reach + width)
-        spans.append((low, high if rows and width else low, block))
-    for at, (low, high, out) in enumerate(spans[:len(results)]):
-        for other_low, other_high, other in spans[at + 1:]:
-            if low < other_high and other_low < high and low < high and other_low < other_high and not (
-                    other is same and out[:3] == other[:3] and (out[1] <= 1 or out[3] == other[3])) and not _beside(
-                    out, other):
-                raise ValueError("%s overlaps %s" % (out[4], other[4]))
-
-
-def _beside(out, other):
-    """Columns of one wider buffer lie between each other without touching."""
-    pitch = out[3]
-    if pitch != other[3] or pitch <= 0:
-        return False
-    gap = (other[0] - out[0]) % pitch
-    return gap >= out[2] and gap + other[2] <= pitch
 
 
 def _number(value, name, low=None, high=None):
