@@ -22,6 +22,12 @@ def from_bfloat16(array):
     return bits.view(np.float32)
 
 
+def host_array(obj, dtype=None):
+    """The compact array of an input on the host.  An empty list holds no integers: NumPy makes float64 of it."""
+    a = np.ascontiguousarray(obj, dtype=dtype)
+    return a if a.size or dtype is not None or hasattr(obj, "dtype") else a.astype(np.int64)
+
+
 def refuse_overlaps(results, inputs, same=None):
     """ValueError when a result array touches an input or another result.  Both are lists of blocks
     (address, rows, bytes of a row, bytes from row to row, name); `same`: the input that a result may

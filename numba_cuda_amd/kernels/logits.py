@@ -29,7 +29,7 @@ import struct
 import numpy as np
 
 from numba_cuda_amd._logits_host import beside as _beside, refuse_overlaps as _refuse_overlaps
-from numba_cuda_amd._logits_host import bfloat16, from_bfloat16, to_bfloat16  # noqa: F401
+from numba_cuda_amd._logits_host import bfloat16, from_bfloat16, host_array, to_bfloat16  # noqa: F401
 from numba_cuda_amd.cudadrv import devicearray, devices
 from numba_cuda_amd.cudadrv import driver as _driver
 
@@ -121,8 +121,7 @@ def _checked_view(obj, name, stream, dtype=None, output=False):
             raise TypeError("%s must be a device array" % name)
         if _capturing(_driver._stream_handle(stream)):       # each replay would copy from a host array that is gone
             raise ValueError("a call that is captured into a graph needs %s in device memory" % name)
-        host = np.ascontiguousarray(obj, dtype=dtype)
-        view = _device_view(devicearray.auto_device(host, stream=stream)[0])
+        view = _device_view(devicearray.auto_device(host_array(obj, dtype), stream=stream)[0])
     if not _one_device() and view[0]:        # memory of another device than the calling thread's
         where, here = ctypes.c_int(), ctypes.c_int()
         _driver.driver.nbh_get_device(ctypes.byref(here))

@@ -6,7 +6,7 @@ import math
 
 import numpy as np
 
-from numba_cuda_amd._logits_host import bfloat16, from_bfloat16, refuse_overlaps, to_bfloat16
+from numba_cuda_amd._logits_host import bfloat16, from_bfloat16, host_array, refuse_overlaps, to_bfloat16
 from numba_cuda_amd.simulator.hostarray import device_array
 
 MOST = 1024
@@ -20,7 +20,7 @@ def _array(obj, dtype=None):
     """The NumPy array of an argument; of an input on the host a compact one, as a copy over is."""
     if getattr(obj, "__cuda_ndarray__", False):
         return obj._ary
-    return np.ascontiguousarray(obj, dtype=dtype)
+    return host_array(obj, dtype)
 
 
 def _address(a):
