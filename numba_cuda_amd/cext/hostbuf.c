@@ -332,7 +332,7 @@ out:
 }
 
 /* The arguments of the row operators (kernels/logits.py), a dozen of which a call of a few
- * microseconds may have: what the Python path (_input / _output with _as_rows or _as_vector)
+ * microseconds may have: what the Python path (_rows_of and _vector_of by way of _checked_view)
  * finds out about an ordinary argument, in one call.  An ordinary argument is an instance of
  * exactly the device array class or of a class listed in `kinds` under its type object, not of a
  * subclass, whose dtype object is a key of `kinds`; the value is (item size, code).  Anything
@@ -340,14 +340,16 @@ out:
  * length, items that do not lie next to each other, an address or row stride that is not a
  * multiple of the item size - gives None, and the Python path takes the argument (and raises
  * what there is to raise).  Torch's strides count items, a device array's bytes: `kinds[type]`
- * is True for the former. */
+ * is True for the former.  A tensor's items have to lie next to each other even where there is one:
+ * those of a negated view (the imaginary part of a conjugated tensor) do not, and the Python
+ * path refuses it. */
 static PyObject *str_is_cuda, *str_dtype, *str_shape, *str_stride, *str_strides, *str_data_ptr, *str_gpu_data,
     *str_device_pointer;
 
 typedef struct {
     unsigned long long address;
     long long shape[2], strides[2]; /* strides in bytes */
-    int ndim;
+    int ndim, tensor;
     long long itemsize;
     PyObject *code; /* borrowed from kinds */
 } plain_view;
@@ -403,6 +405,7 @@ static int plain_view_of(PyObject *obj, PyObject *kinds, plain_view *v)
     v->itemsize = PyLong_AsLongLong(PyTuple_GET_ITEM(kind, 0));
     v->code = PyTuple_GET_ITEM(kind, 1);
     v->ndim = (int)PyTuple_GET_SIZE(shape);
+    v->tensor = tensor;
     for (int k = 0; k < v->ndim; ++k) {
         v->shape[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(shape, k));
         v->strides[k] = PyLong_AsLongLong(PyTuple_GET_ITEM(strides, k)) * (tensor ? v->itemsize : 1);
@@ -428,7 +431,7 @@ static PyObject *hb_row_view(PyObject *mod, PyObject *const *args, Py_ssize_t na
     const int rc = plain_view_of(args[0], args[1], &v);
     if (rc < 0)
         return NULL;
-    if (rc || v.ndim != 2 || (v.shape[1] > 1 && v.strides[1] != v.itemsize) || v.address % v.itemsize ||
+    if (rc || v.ndim != 2 || ((v.shape[1] > 1 || v.tensor) && v.strides[1] != v.itemsize) || v.address % v.itemsize ||
         (v.shape[0] > 1 && v.strides[0] % v.itemsize))
         Py_RETURN_NONE;
     return Py_BuildValue("KLLLO", v.address, v.shape[0], v.shape[1], v.shape[0] > 1 ? v.strides[0] : 0LL, v.code);
@@ -449,7 +452,7 @@ static PyObject *hb_vector_view(PyObject *mod, PyObject *const *args, Py_ssize_t
     if (rc < 0)
         return NULL;
     if (rc || v.ndim != 1 || (length >= 0 && v.shape[0] != length) ||
-        (v.shape[0] > 1 && v.strides[0] != v.itemsize) || v.address % v.itemsize)
+        ((v.shape[0] > 1 || v.tensor) && v.strides[0] != v.itemsize) || v.address % v.itemsize)
         Py_RETURN_NONE;
     return Py_BuildValue("KLL", v.address, v.shape[0], v.itemsize);
 }

@@ -96,6 +96,8 @@ def _device_view(obj):
     if _is_tensor(obj):
         if not obj.is_cuda:
             return None
+        if getattr(obj, "is_neg", bool)():
+            raise TypeError("the tensor is a negated view of its memory: torch.resolve_neg makes an ordinary one")
         dtype = _foreign_dtypes.get(obj.dtype) or _foreign_dtype(obj.dtype)
         return obj.data_ptr(), tuple(obj.shape), tuple([n * dtype.itemsize for n in obj.stride()]), dtype, obj
     if hasattr(obj, "__cuda_array_interface__"):
