@@ -534,10 +534,16 @@ template <typename E> __global__ __launch_bounds__(256) void distill_named(Disti
 // 8192 40, 40 and 74.  In several launches: loss 131072 x 1024 280 instead of 171, 16384 x 8192 70 instead of 59,
 // gradient 288 instead of 234 and 153 instead of 137.
 // Both at once, 256 and 512 lanes: 4096 x 16384 67 and 97, 4096 x 32768 125 and 130, 512 x 16384 17 and 17, 256 x
-// 32768 18 and 17, 4096 x 50021 242 and 224, 4096 x 65536 244 and 209.  With many entries of the teacher, whose LDS
-// leaves room for one workgroup of 512 only and which take a wavefront long: 4096 x 65536, k = 150 267 and 256, 300
-// 299 and 317, 500 347 and 415, 600 371 and 627, 1000 457 and 906; 1024 x 131072, k = 300 149 and 137, 500 166 and
-// 174, 1000 205 and 287; 256 x 131072, k = 1000 77 and 71.
+// 32768 18 and 17, 4096 x 50021 242 and 224, 4096 x 65536 239 and 206.  Many entries of the teacher take a wavefront
+// long, which more rows under way hide better, unless the row is longer than what 512 lanes keep of it; of more than
+// 512 entries LDS leaves room for one workgroup of 512 only.  k = 64, 150, 250, 300, 350, 400 and 512:
+//   4096 x 65536 bfloat16   239 256 276 291 311 331 359 and 206 264 304 321 349 387 451
+//   1024 x 50021 float16     61  66  71  73  76  79  83 and  53  61  69  71  76  80  89
+//   600 x 32768 float32      39  45  48  50  52  54  59 and  35  44  51  53  57  62  70
+//   2048 x 65536 float32    234 246 259 268 275 284 308 and 209 231 255 263 275 288 309
+//   1024 x 131072 bfloat16  121 131 141 146 152 157 164 and  97 110 124 128 138 147 160
+//   512 x 65536 bfloat16     35  41  44  45  48  50  54 and  27  33  37  39  42  45  49
+//   k = 600 4096 x 65536 371 and 627, 1000 457 and 906, 1024 x 131072 205 and 287, 256 x 131072 77 and 71.
 enum Way { kRows, kInParts, kFlat };
 struct Spread {
     Way way;
@@ -561,7 +567,7 @@ Spread spread_of(int64_t rows, int64_t vocab, int64_t k, int dtype, int what, in
     if (what == kLoss)
         return {large || (rows < 256 && chunks > 24) ? kInParts : kRows, tiles, small ? 64 : 256, 1, vocab};
     if (what == (kLoss | kGrad) && (rows >= 128 || chunks <= 12)) {
-        const bool more = (chunks <= 4 && rows > 512) || (k > 512 && rows > 256);
+        const bool more = (rows > 512 && (chunks <= 4 || (k > 300 && chunks <= 10))) || (k > 512 && rows > 256);
         return {kRows, tiles, small ? 64 : more ? 256 : 512, 1, vocab};
     }
     int64_t splits = (1024 + rows - 1) / rows;
