@@ -14,8 +14,8 @@
 //
 // Bound by memory: the loss reads a row once (2048 x 50021 float16: 36 + 6 us, 205 MB at 5.8 TB/s in the first
 // launch), the gradient reads and writes it (1024 x 100003 float32: 10 + 139 + 5 us, 819 MB at 5.9 TB/s in the
-// second).  Both at once read it once and the part that was not kept again (4096 x 131072 bfloat16: 415 us; 1.35 GB
-// read and 1.08 GB written leave or enter the L2 caches, 5.9 TB/s); beside the traffic there are two exponentials
+// second).  Both at once read it once and the part that was not kept again (4096 x 131072 bfloat16: 414 us; 1.33 GB
+// read and 1.08 GB written leave or enter the L2 caches, 5.8 TB/s); beside the traffic there are two exponentials
 // per entry, some 0.28 ms of the vector units' time.
 #include "rows.h"
 

@@ -241,6 +241,9 @@ int launch_adjust(const Adjust &a, int64_t rows, hipStream_t stream)
     // 17.4 and 18.9 us, 256 rows 48 and 55; 16384: 64 rows 22.8 and 20.6, 256 rows 62 and 64; 65536: 1 row 34 and
     // 16, 64 rows 64 and 40, 256 rows 164 and 125.  (8 rows of 131072 float32, 65536: tiles of 16384 18.8 us, of
     // 8192 16.7, of 32768 21.9.)
+    // Only the mean is known here, the lengths are on the device.  One history of 131071 among rows of 100 tokens
+    // waits for its 32 workgroups: 16 rows 32 and 14.5 us, 64 rows 67 and 31, 256 rows 69 and 47; of 16384 64 rows
+    // 14.5 and 12.9, 256 rows 24 and 30.
     if (a.n_tokens / rows > 12288)
         return launch_adjust<In, Out, 1024, 8192>(a, rows, stream);
     return launch_adjust<In, Out, 256, 4096>(a, rows, stream);

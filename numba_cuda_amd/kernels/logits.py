@@ -16,7 +16,9 @@ float32, float16 or bfloat16, which NumPy has no type for: two-byte void items (
 the type string "<V2") are bfloat16.  Items of a row lie next to each other; rows may be any multiple
 of the item size apart.  Arithmetic is float32, results are rounded once.
 
-Everything is asynchronous on `stream`, and results do not depend on how the work was spread.  A call
+Everything is asynchronous on `stream`.  Results are the same from call to call.  Sums are formed in an
+order that goes by the number of rows, their length and alignment, so the last bits of lse, loss and
+gradients of a row depend on the array it is in; `adjust` and the entries of `top` do not.  A call
 that needs a workspace keeps one per stream; a call recorded into a graph takes the caller's
 (`workspace=`, at least `top_workspace` / `distill_workspace` bytes) and the caller's result arrays,
 since a graph may run beside later calls on its stream, and inputs in device memory only.
